@@ -1,0 +1,183 @@
+// Differential attention: shared pieces of its kernels (diff_attn.hip, diff_attn_bwd.hip).  gfx950 only.
+//
+//   o = (softmax(s q1 k1^T) - lam softmax(s q2 k2^T)) v        per segment and head; d columns per map, 2d columns of v
+//
+// Everything is written on 16 x 16 matrix-instruction tiles with a contraction of 32 and ONE fragment layout: lane l holds
+// eight elements of row (A) or column (B) l & 15, the contraction slots (l >> 4) * 8 + j.  16-bit types take one
+// v_mfma_f32_16x16x32; fp32 takes eight v_mfma_f32_16x16x4_f32, the j-th on element j of every lane (a contraction may be
+// summed in any order as long as both operands agree on it), so fp32 inputs keep fp32 products.
+// A result tile has column l & 15 and rows (l >> 4) * 4 + r in register r.  Two result tiles of one column block, converted,
+// ARE a B fragment over their 32 rows if slot (g, j) is read as row g * 4 + j (j < 4) or 16 + g * 4 + j - 4: attention
+// weights feed the next product from the registers they were computed in.  The other operand of that product is then a
+// matrix read down its columns: ds_read_b64_tr_b16 hands lane l the four elements (g * 4 .. g * 4 + 3, l & 15) of a row-major
+// LDS tile, which is that slot order.
+#pragma once
+#include "gps_common.hpp"
+
+namespace diffattn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+template <typename T, int N>
+using vec_t = T __attribute__((ext_vector_type(N)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kInf = __builtin_huge_valf();
+
+using Args = gps_diff_attn;   // include/gps_hip.h
+
+template <typename T>
+struct Frag {
+  vec_t<T, 8> v;
+};
+template <>
+struct Frag<float> {
+  f32x4 lo, hi;
+};
+
+__device__ __forceinline__ f32x4 mma(const Frag<bf16>& a, const Frag<bf16>& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Frag<f16>& a, const Frag<f16>& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[j], b.lo[j], c, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[j], b.hi[j], c, 0, 0, 0);
+  return c;
+}
+
+// eight contiguous elements at p (16-byte aligned; global or LDS)
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_load(const T* p) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 4) {
+    f.lo = *reinterpret_cast<const f32x4*>(p);
+    f.hi = *reinterpret_cast<const f32x4*>(p + 4);
+  } else {
+    f.v = *reinterpret_cast<const vec_t<T, 8>*>(p);
+  }
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_zero() {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 4) {
+    f.lo = f32x4{0.f, 0.f, 0.f, 0.f};
+    f.hi = f.lo;
+  } else {
+    f.v = vec_t<T, 8>(0);
+  }
+  return f;
+}
+// two result tiles -> the B fragment over their 32 rows.  16-bit types round to nearest here: the weights and their
+// gradients enter the second product in the input's type, which is what the matrix instruction takes.
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_pack(f32x4 a, f32x4 b) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 4) {
+    f.lo = a;
+    f.hi = b;
+  } else {
+    const vec_t<T, 4> x = __builtin_convertvector(a, vec_t<T, 4>), y = __builtin_convertvector(b, vec_t<T, 4>);
+    f.v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+// A fragment of the TRANSPOSE of the row-major LDS tile `m` (row stride `ld`): row of A = column col0 + (l & 15), slots = rows
+// row0 .. row0 + 31 in frag_pack's order
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_tr(const T* m, int ld, int row0, int col0, int lane) {
+  Frag<T> f;
+  const int g = lane >> 4, i = lane & 15;
+  if constexpr (sizeof(T) == 4) {
+    const float* p = m + (row0 + g * 4) * ld + col0 + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f.lo[j] = p[j * ld];
+      f.hi[j] = p[(16 + j) * ld];
+    }
+  } else {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    T* p = const_cast<T*>(m) + (row0 + g * 4 + (i >> 2)) * ld + col0 + (i & 3) * 4;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 16 * ld));
+    f.v = __builtin_bit_cast(vec_t<T, 8>, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  return f;
+}
+
+// four results -> four contiguous elements of T at p (aligned to four elements)
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 x) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<f32x4*>(p) = x;
+  else
+    *reinterpret_cast<vec_t<T, 4>*>(p) = __builtin_convertvector(x, vec_t<T, 4>);
+}
+
+__device__ __forceinline__ float load_lam(const Args& a, int h, const bf16*) {
+  return a.lam_f32 ? static_cast<const float*>(a.lam)[h] : (float)static_cast<const bf16*>(a.lam)[h];
+}
+__device__ __forceinline__ float load_lam(const Args& a, int h, const f16*) {
+  return a.lam_f32 ? static_cast<const float*>(a.lam)[h] : (float)static_cast<const f16*>(a.lam)[h];
+}
+__device__ __forceinline__ float load_lam(const Args& a, int h, const float*) { return static_cast<const float*>(a.lam)[h]; }
+
+__device__ __forceinline__ int clamp_row(int32_t r, int64_t n) { return r < 0 ? 0 : (r > n ? (int)n : r); }
+
+// Which rows tile `tile` covers, without a tile map and without the host knowing the segment lengths.  Segment s owns the tile
+// numbers from ptr[s] / bm + s on: that grows by at least ceil(length / bm) from each segment to the next and never passes
+// N / bm + B, so N / bm + B + 1 tiles cover every segment and the rows behind the last one (segment B).  64 lanes probe at a
+// time: two rounds for up to 4,096 segments.  Lane-uniform.  Entries outside [0, N] are cut to it: no row index leaves N.
+struct Tile {
+  int seg, first, rows;  // segment (B = behind the last one), first row, rows in this tile (<= 0: none)
+  int local;             // index of `first` in the segment
+  int len;               // rows of the segment
+};
+__device__ __forceinline__ Tile find_tile(const int32_t* ptr, int B, int64_t N, int bm, int tile) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = B;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) >> 6;
+    const int s = lo + (lane + 1) * step;
+    bool in = false;
+    if (s <= hi) in = clamp_row(ptr[s], N) / bm + s <= tile;
+    const int n = __popcll(__ballot(in));
+    lo += n * step;
+    hi = min(hi, lo + step - 1);
+  }
+  Tile t;
+  t.seg = __builtin_amdgcn_readfirstlane(lo);
+  const int begin = clamp_row(ptr[t.seg], N);
+  const int end = t.seg < B ? clamp_row(ptr[t.seg + 1], N) : (int)N;
+  t.local = (tile - (begin / bm + t.seg)) * bm;
+  t.first = begin + t.local;
+  t.rows = t.local < 0 ? 0 : min(bm, end - t.first);
+  t.len = max(0, end - begin);
+  return t;
+}
+
+// rows [row0, row0 + n) of `src` (C columns of which `cols` exist, both multiples of 8) -> row-major LDS tile of R rows, stride
+// `ld`; rows past `n` and those that ok(r) refuses, and columns past `cols`, are zero: whatever a dropped row holds, 0 * it is
+// never formed.
+template <typename T, int R, int C, typename Ok>
+__device__ __forceinline__ void stage(T* dst, int ld, const T* src, int64_t row_stride, int n, int cols, Ok ok) {
+  constexpr int kEl = 16 / sizeof(T), kPer = C / kEl;
+  for (int i = threadIdx.x; i < R * kPer; i += blockDim.x) {
+    const int r = i / kPer, c = (i % kPer) * kEl;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < n && c < cols && ok(r)) x = *reinterpret_cast<const uint4*>(src + r * row_stride + c);
+    *reinterpret_cast<uint4*>(dst + r * ld + c) = x;
+  }
+}
+
+template <typename T>
+void backward(const Args& a, hipStream_t s);   // diff_attn_bwd.hip
+
+}  // namespace diffattn

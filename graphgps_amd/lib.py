@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from typing import Optional
 
 import torch  # noqa: F401  -- must be imported first: it maps the HIP runtime our .so binds to
@@ -15,7 +15,7 @@ import torch  # noqa: F401  -- must be imported first: it maps the HIP runtime o
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # GPS_HIP_LIB: an alternative build of the same ABI (A/B timing of kernel variants in one process launch each)
 LIB_PATH = os.environ.get("GPS_HIP_LIB") or os.path.join(_HERE, "csrc", "libgps_hip.so")
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -126,6 +126,17 @@ _SIGNATURES = {
     "gps_adj_sum": (c_int, [_P, c_int64, _P, _P, c_float, c_int64, c_int64, c_int, _P, _P]),
     "gps_seg_attn_bias_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, c_int64, c_int64, c_int, c_int,
                                       c_float, c_float, c_uint64, _P, _P, _P]),
+    "gps_diff_attn_bwd_workspace_floats": (c_size_t, [c_int64, c_int]),
+    "gps_diff_attn_fwd": (c_int, [_P, _P]),
+    "gps_diff_attn_bwd": (c_int, [_P, _P]),
+    "gps_sandwich_max_width": (c_int, []),
+    "gps_sandwich_workspace_floats": (c_size_t, [c_int64, c_int]),
+    "gps_sandwich_norm_fwd": (c_int, [_P, _P]),
+    "gps_sandwich_norm_bwd": (c_int, [_P, _P]),
+    "gps_adamw8_block": (c_int, []),
+    "gps_adamw8_workspace_floats": (c_size_t, [c_int64]),
+    "gps_adamw8_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P, _P, c_uint32, _P, _P]),
+    "gps_adamw8_values": (c_int, [_P, _P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, _P, _P, _P]),
     "gps_seg_attn_bias_bwd": (c_int, [_P, _P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64,
                                       c_int, c_int, c_float, c_float, c_uint64, _P, _P, c_int64, _P, _P]),
 }
@@ -182,6 +193,29 @@ class GemmSplit16(ctypes.Structure):
     """``gps_gemm_split16`` (include/gps_hip.h)."""
     _fields_ = [("W", c_void_p), ("ldw", c_int64), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
                 ("image_nt", c_void_p), ("image_tn", c_void_p), ("amax", c_void_p)]
+
+
+class DiffAttn(ctypes.Structure):
+    """``gps_diff_attn`` (include/gps_hip.h)."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "lam")]
+                + [(n, c_int64) for n in ("q_rs", "q_hs", "q_ms", "k_rs", "k_hs", "k_ms", "v_rs", "v_hs")]
+                + [(n, c_void_p) for n in ("q_ptr", "k_ptr", "keep")] + [("Nq", c_int64), ("Nk", c_int64)]
+                + [(n, c_int32) for n in ("B", "H", "Hk", "d", "causal", "lam_f32", "dtype", "max_q", "max_k")]
+                + [("scale", c_float)] + [(n, c_void_p) for n in ("o", "o2", "lse", "dout")]
+                + [("do_rs", c_int64), ("do_hs", c_int64)] + [(n, c_void_p) for n in ("dq", "dk", "dv", "dlam")]
+                + [(n, c_int64) for n in ("dq_rs", "dq_hs", "dq_ms", "dk_rs", "dk_hs", "dk_ms", "dv_rs", "dv_hs")]
+                + [("ws", c_void_p), ("ws_floats", c_size_t)])
+
+
+class SandwichNorm(ctypes.Structure):
+    """``gps_sandwich_norm`` (include/gps_hip.h)."""
+    _fields_ = ([(n, c_void_p) for n in ("a", "x", "gate_full")] + [(n, c_int64) for n in ("a_rs", "x_rs", "g_rs")]
+                + [(n, c_void_p) for n in ("post_weight", "post_bias", "pre_weight", "pre_bias", "gate")]
+                + [("N", c_int64)] + [(n, c_int32) for n in ("D", "kind", "dtype")]
+                + [(n, c_float) for n in ("alpha", "beta", "eps")] + [(n, c_void_p) for n in ("y", "z", "stats", "dy", "dz")]
+                + [("dy_rs", c_int64), ("dz_rs", c_int64)] + [(n, c_void_p) for n in ("dx", "da", "dgate_full")]
+                + [(n, c_void_p) for n in ("dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias", "dgate", "ws")]
+                + [("ws_floats", c_size_t)])
 
 
 class GpsHipError(RuntimeError):

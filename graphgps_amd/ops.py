@@ -820,3 +820,10 @@ def embedding(idx: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
             and weight.is_contiguous():
         return _Embedding.apply(idx.contiguous(), weight)
     return torch.nn.functional.embedding(idx, weight)
+
+
+# -------------------------------------------------------------------------------------------
+# differential attention, the residual stream of a block
+# -------------------------------------------------------------------------------------------
+from .diff_attention import diff_attention, diff_segment_attention  # noqa: E402,F401
+from .sandwich import sandwich_norm  # noqa: E402,F401

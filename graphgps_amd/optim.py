@@ -246,15 +246,18 @@ class FlatAdamW(torch.optim.Optimizer):
             raise ValueError("FlatAdamW supports a single parameter group")
         self.arena = ParamArena(params)
         dev = self.arena.device
-        n = self.arena.flat_p.numel()
-        self.exp_avg = torch.zeros(n, dtype=torch.float32, device=dev)
-        self.exp_avg_sq = torch.zeros(n, dtype=torch.float32, device=dev)
+        self._alloc_state()
         self.hyper = torch.zeros(8, dtype=torch.float64, device=dev)
         self.param_step = torch.zeros(len(self.arena.params), dtype=torch.float32, device=dev)
-        self._ws = torch.empty(max(self.arena.n_chunks, 1), dtype=torch.float32, device=dev)
         self._hyper_host = None
         self._packed = False
         self.sync_hyper()
+
+    def _alloc_state(self) -> None:
+        n, dev = self.arena.flat_p.numel(), self.arena.device
+        self.exp_avg = torch.zeros(n, dtype=torch.float32, device=dev)
+        self.exp_avg_sq = torch.zeros(n, dtype=torch.float32, device=dev)
+        self._ws = torch.empty(max(self.arena.n_chunks, 1), dtype=torch.float32, device=dev)
 
     # ------------------------------------------------------------------ hyper-parameters
     def _hyper_tuple(self):
@@ -327,14 +330,18 @@ class FlatAdamW(torch.optim.Optimizer):
             self.pack_grads()
         if not torch.cuda.is_current_stream_capturing():
             self.sync_hyper()
+        self._launch_step()
+        self._packed = False
+        return loss
+
+    def _launch_step(self) -> None:
+        a = self.arena
         check(_lib.load().gps_adamw_step(ptr(a.flat_p), ptr(a.flat_g), ptr(self.exp_avg),
                                          ptr(self.exp_avg_sq), ptr(a.chunk_off), ptr(a.chunk_len),
                                          ptr(a.chunk_param), ptr(a.active), a.n_chunks,
                                          ptr(self.hyper), ptr(self.param_step), ptr(self._ws),
                                          current_stream(a.device)),
               "gps_adamw_step")
-        self._packed = False
-        return loss
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         # gradients are re-packed every step, so dropping the references is all there is to do
@@ -387,12 +394,180 @@ class FlatAdamW(torch.optim.Optimizer):
         self.sync_hyper()
 
 
+class FlatAdamW8bit(FlatAdamW):
+    """:class:`FlatAdamW` with both moments held in 8 bits (csrc/optim8.hip): 2 bytes of state per parameter instead of 8, and
+    20 bytes of traffic per parameter and step instead of 32.
+
+    A moment is a byte per element plus a power-of-two unit per block of 256 elements of a parameter (codes of three mantissa bits;
+    include/gps_hip.h has the format).  Codes are rounded up or down at random so that the moving averages keep their mean; the
+    random bits are a hash of (element, step, ``seed``), so a run repeats exactly.  Parameters, gradients and the update itself are
+    fp32.  A gradient that is not finite makes the moments of its whole block so.
+
+    ``state_dict()`` holds the codes (uint8 ``exp_avg`` / ``exp_avg_sq`` in the parameter's shape, their blocks' ``*_exp``);
+    ``load_state_dict()`` takes those, or the fp32 moments of :class:`FlatAdamW` / ``torch.optim.AdamW`` and rounds them to
+    nearest."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 max_grad_norm: Optional[float] = None, seed: int = 0):
+        if not 0 <= int(seed) < 1 << 32:
+            raise ValueError(f"FlatAdamW8bit: seed {seed} is no 32-bit unsigned number")
+        super().__init__(params, lr, betas, eps, weight_decay, max_grad_norm)
+        self.seed = int(seed)
+
+    def _alloc_state(self) -> None:
+        a = self.arena
+        n = a.flat_p.numel()
+        self.block = _lib.load().gps_adamw8_block()
+        blocks = a.n_chunks * (_lib.load().gps_optim_chunk() // self.block)
+        u8 = dict(dtype=torch.uint8, device=a.device)
+        self.exp_avg, self.exp_avg_sq = torch.zeros(n, **u8), torch.zeros(n, **u8)
+        self.exp_avg_exp, self.exp_avg_sq_exp = torch.zeros(blocks, **u8), torch.zeros(blocks, **u8)
+        self._alloc_tables()
+
+    def _alloc_tables(self) -> None:
+        """What depends on the arena's layout: the workspace and the pieces of the arena that belong to no parameter."""
+        a, L = self.arena, _lib.load()
+        self._ws = torch.empty(max(int(L.gps_adamw8_workspace_floats(a.n_chunks)), 1), dtype=torch.float32, device=a.device)
+        step, at, gaps = L.gps_optim_chunk(), 0, []
+        for o, k in sorted((o, p.numel()) for o, p in zip(a.offsets, a.params)) + [(a.flat_p.numel(), 0)]:
+            if o < at and k:
+                raise ValueError("FlatAdamW8bit: two parameters share elements; their codes would not fit both blocks' units")
+            gaps += [(s, min(step, o - s)) for s in range(at, o, step)]
+            at = max(at, o + k)
+        self._gap_off = torch.tensor([g[0] for g in gaps], dtype=torch.int64, device=a.device)
+        self._gap_len = torch.tensor([g[1] for g in gaps], dtype=torch.int32, device=a.device)
+
+    def _readopt(self) -> None:
+        m, v = self.exp_avg, self.exp_avg_sq
+        old = self.arena.adopt()
+        n = self.arena.flat_p.numel()
+        self.exp_avg = torch.zeros(n, dtype=torch.uint8, device=self.arena.device)
+        self.exp_avg_sq = torch.zeros_like(self.exp_avg)
+        for o_old, o_new, p in zip(old, self.arena.offsets, self.arena.params):
+            k = p.numel()
+            self.exp_avg[o_new:o_new + k].copy_(m[o_old:o_old + k])
+            self.exp_avg_sq[o_new:o_new + k].copy_(v[o_old:o_old + k])
+        self._alloc_tables()          # the blocks' exponents go by chunk number, which a move leaves as it was
+
+    def _launch_step(self) -> None:
+        a = self.arena
+        with torch.cuda.device(a.device):
+            check(_lib.load().gps_adamw8_step(ptr(a.flat_p), ptr(a.flat_g), ptr(self.exp_avg), ptr(self.exp_avg_sq),
+                                              ptr(self.exp_avg_exp), ptr(self.exp_avg_sq_exp), ptr(a.chunk_off), ptr(a.chunk_len),
+                                              ptr(a.chunk_param), ptr(a.active), a.n_chunks, ptr(self.hyper), ptr(self.param_step),
+                                              self.seed, ptr(self._ws), current_stream(a.device)), "gps_adamw8_step")
+
+    def moments(self, dtype: torch.dtype = torch.bfloat16):
+        """``(exp_avg, exp_avg_sq)`` as numbers, in the arena's layout (``arena.offsets``); bfloat16 holds every value exactly."""
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise _lib.GpsHipError(f"FlatAdamW8bit.moments: {dtype} is neither bfloat16 nor float32")
+        a = self.arena
+        m = torch.empty(a.flat_p.numel(), dtype=dtype, device=a.device)
+        v = torch.empty_like(m)
+        with torch.cuda.device(a.device):
+            check(_lib.load().gps_adamw8_values(ptr(self.exp_avg), ptr(self.exp_avg_sq), ptr(self.exp_avg_exp),
+                                                ptr(self.exp_avg_sq_exp), ptr(a.chunk_off), ptr(a.chunk_len), a.n_chunks,
+                                                ptr(self._gap_off), ptr(self._gap_len), self._gap_off.numel(),
+                                                1 if dtype == torch.bfloat16 else 0, ptr(m), ptr(v), current_stream(a.device)),
+                  "gps_adamw8_values")
+        return m, v
+
+    # ------------------------------------------------------------------ checkpointing
+    def _block_ranges(self):
+        """Per parameter: its slice of the blocks' exponents (chunks follow the parameters' order, only a last one is short)."""
+        per, at, out = _lib.load().gps_optim_chunk(), 0, []
+        for p in self.arena.params:
+            n = p.numel()
+            chunks = -(-n // per)
+            out.append((at * (per // self.block), -(-n // self.block)))
+            at += chunks
+        return out
+
+    def state_dict(self):
+        a = self.arena
+        steps = self.param_step.detach().cpu()
+        state = {}
+        for i, (o, p, (b, nb)) in enumerate(zip(a.offsets, a.params, self._block_ranges())):
+            if float(steps[i]) == 0.0:
+                continue
+            k = p.numel()
+            state[i] = dict(step=steps[i].clone(), exp_avg=self.exp_avg[o:o + k].view(p.shape).clone(),
+                            exp_avg_sq=self.exp_avg_sq[o:o + k].view(p.shape).clone(),
+                            exp_avg_exp=self.exp_avg_exp[b:b + nb].clone(), exp_avg_sq_exp=self.exp_avg_sq_exp[b:b + nb].clone())
+        g = {k: v for k, v in self.param_groups[0].items() if k != "params"}
+        g["params"] = list(range(len(a.params)))
+        return {"state": state, "param_groups": [g], "seed": self.seed}
+
+    @torch.no_grad()
+    def load_state_dict(self, sd) -> None:
+        a = self.arena
+        for k, v in sd["param_groups"][0].items():
+            if k != "params":
+                self.param_groups[0][k] = v
+        self.param_groups[0].setdefault("max_grad_norm", None)
+        self.seed = int(sd.get("seed", self.seed))
+        steps = [0.0] * len(a.params)
+        for t in (self.exp_avg, self.exp_avg_sq, self.exp_avg_exp, self.exp_avg_sq_exp):
+            t.zero_()
+        for i, (o, p, (b, nb)) in enumerate(zip(a.offsets, a.params, self._block_ranges())):
+            st = sd["state"].get(i)
+            if st is None:
+                continue
+            k = p.numel()
+            for name, octaves in (("exp_avg", 18), ("exp_avg_sq", 34)):
+                code = st[name].reshape(-1).to(a.device)
+                if code.numel() != k:
+                    raise ValueError(f"FlatAdamW8bit: {name} of parameter {i} has {code.numel()} elements, not {k}")
+                if code.dtype == torch.uint8:
+                    exp = st[name + "_exp"].reshape(-1)
+                    if exp.numel() != nb:
+                        raise ValueError(f"FlatAdamW8bit: {name}_exp of parameter {i} has {exp.numel()} blocks, not {nb}")
+                else:
+                    code, exp = encode_moment(code.float(), octaves, self.block)
+                getattr(self, name)[o:o + k].copy_(code)
+                getattr(self, name + "_exp")[b:b + nb].copy_(exp)
+            steps[i] = float(st["step"])
+        self.param_step.copy_(torch.tensor(steps, dtype=torch.float32))
+        self.hyper[6] = max(steps)
+        self._hyper_host = None
+        self.sync_hyper()
+
+
+def encode_moment(x: torch.Tensor, octaves: int, block: int = 256):
+    """fp32 values -> (codes, exponents of their blocks) of the 8-bit moments, rounded to nearest (include/gps_hip.h has the format;
+    ``octaves`` 18: signed, ``exp_avg``; 34: ``exp_avg_sq``).  For loading fp32 state: the step itself encodes in its kernel."""
+    n = x.numel()
+    y = torch.nn.functional.pad(x, (0, -n % block)).view(-1, block)
+    size = y.abs()
+    top = size.amax(-1)
+    frac, e = torch.frexp(top)
+    k = (e + (frac > 0.9375) - octaves).clamp(min=-126)
+    units = size * ((127 - k) << 23).to(torch.int32).view(torch.float32)[:, None]
+    small = torch.floor(units + 0.5).to(torch.int32)
+    large = ((units.view(torch.int32) + (1 << 19)) >> 20) - 1032
+    code = torch.where(units < 8, small, large)
+    if octaves == 34:
+        code = torch.where((code == 0) & (units > 0), 1, code)
+    else:
+        code = code | ((y < 0) & (code > 0)).to(torch.int32) << 7
+    fine = torch.isfinite(top)
+    code = torch.where(fine[:, None], code, 0).to(torch.uint8).view(-1)[:n]
+    exp = torch.where(fine, torch.where(top == 0, 0, k + 127), 255).to(torch.uint8)
+    return code, exp
+
+
 def adamW_optimizer(params, base_lr: float, weight_decay: float,
                     max_grad_norm: Optional[float] = None) -> FlatAdamW:
     """``register_optimizer('adamW')`` (extra_optimizers.py:21-24), same signature."""
     return FlatAdamW(params, lr=base_lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
 
 
+def adamW8bit_optimizer(params, base_lr: float, weight_decay: float, max_grad_norm: Optional[float] = None) -> FlatAdamW8bit:
+    """``optim.optimizer: adamW8bit``: the ``adamW`` signature over 8-bit moments."""
+    return FlatAdamW8bit(params, lr=base_lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
+
+
 from .graphgym import register as _register  # noqa: E402
 
 _register.register_optimizer('adamW', adamW_optimizer, overwrite=True)
+_register.register_optimizer('adamW8bit', adamW8bit_optimizer, overwrite=True)

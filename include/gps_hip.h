@@ -726,6 +726,105 @@ int gps_adamw_step(float* p, const float* g, float* m, float* v, const int64_t* 
                    const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active,
                    int64_t n_chunks, double* hyper, float* pstep, float* ws, gps_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Differential attention over ragged segments:
+ *   o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v     per segment and head, lam per head
+ * q [Nq, H, 2, d], k [Nk, Hk, 2, d], v [Nk, Hk, 2d] by element strides (last dimension contiguous), H a multiple of Hk: head h
+ * reads key head h / (H / Hk).  Segment s owns the query rows q_ptr[s] .. q_ptr[s+1] and the key rows k_ptr[s] .. k_ptr[s+1]
+ * (int32 [B+1], non-decreasing from 0; entries outside the rows are cut to them); rows behind the last segment, and rows that see
+ * no key, give o = 0 and gradients of 0.  causal: the query at index i of a segment with n queries and m keys sees the keys
+ * 0 .. i + m - n.  keep [Nk] bytes, 0 = dropped key (what its rows of k and v hold is not read); NULL = none dropped.
+ * dtype of q, k, v, o and of the gradients: GPS_F32, GPS_BF16 or GPS_F16; sums and softmax statistics are fp32.  lam is fp32
+ * (lam_f32 != 0) or of that dtype, and so is its gradient.  d a multiple of 8, at most 128; base pointers 16-byte aligned and
+ * row / head / map strides multiples of 8 elements.  max_q / max_k: the longest segment if the host knows it, else 0; they choose
+ * the launch shape only.
+ * Training keeps o2 [Nq, H, 2d] (fp32, the second map's share of o) and lse [2, H, Nq] (fp32); both NULL at inference.
+ * Backward workspace: gps_diff_attn_bwd_workspace_floats().  The results do not depend on how work is split: no atomics. */
+#define GPS_F32 0
+#define GPS_BF16 1
+#define GPS_F16 2
+typedef struct gps_diff_attn {
+  const void *q, *k, *v, *lam;
+  int64_t q_rs, q_hs, q_ms, k_rs, k_hs, k_ms, v_rs, v_hs; /* row, head, map */
+  const int32_t *q_ptr, *k_ptr;
+  const uint8_t* keep;
+  int64_t Nq, Nk;
+  int32_t B, H, Hk, d, causal, lam_f32, dtype, max_q, max_k;
+  float scale;
+  void* o; /* [Nq, H, 2d] contiguous */
+  float* o2;
+  float* lse;
+  /* backward only */
+  const void* dout;
+  int64_t do_rs, do_hs;
+  void *dq, *dk, *dv, *dlam;
+  int64_t dq_rs, dq_hs, dq_ms, dk_rs, dk_hs, dk_ms, dv_rs, dv_hs;
+  float* ws;
+  size_t ws_floats;
+} gps_diff_attn;
+
+size_t gps_diff_attn_bwd_workspace_floats(int64_t Nq, int H);
+int gps_diff_attn_fwd(const gps_diff_attn* a, gps_stream_t stream);
+int gps_diff_attn_bwd(const gps_diff_attn* a, gps_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The residual stream of a block in one pass:  n = norm(a; post),  y = alpha x + beta gate o n,  z = norm(y; pre).
+ * Rows of a, x, gate_full, dy, dz by row stride (elements), contiguous within the row; y, z, dx, da, dgate_full contiguous
+ * [N, D].  dtype is theirs; all parameters and parameter gradients are fp32 [D].  A NULL post_weight / pre_weight leaves that
+ * norm out (n = a / no z); NULL biases, gate and x are left out too; gate is a channel vector, gate_full a matrix.
+ * Training keeps stats [4, N] (fp32: mean and reciprocal deviation of the two norms).  Backward: dy or dz may be NULL (zero);
+ * any output gradient but da may be NULL (not wanted).  ws: gps_sandwich_workspace_floats().  D <= gps_sandwich_max_width().
+ * Sums are in a fixed order: no atomics. */
+#define GPS_NORM_RMS 0
+#define GPS_NORM_LAYER 1
+typedef struct gps_sandwich_norm {
+  const void *a, *x, *gate_full;
+  int64_t a_rs, x_rs, g_rs;
+  const float *post_weight, *post_bias, *pre_weight, *pre_bias, *gate;
+  int64_t N;
+  int32_t D, kind, dtype;
+  float alpha, beta, eps;
+  void *y, *z;
+  float* stats;
+  /* backward only */
+  const void *dy, *dz;
+  int64_t dy_rs, dz_rs;
+  void *dx, *da, *dgate_full;
+  float *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias, *dgate;
+  float* ws;
+  size_t ws_floats;
+} gps_sandwich_norm;
+
+int gps_sandwich_max_width(void);
+size_t gps_sandwich_workspace_floats(int64_t N, int D);
+int gps_sandwich_norm_fwd(const gps_sandwich_norm* a, gps_stream_t stream);
+int gps_sandwich_norm_bwd(const gps_sandwich_norm* a, gps_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Clip + AdamW over the arena of gps_adamw_step with both moments in 8 bits: 1 byte per element and moment plus 1 byte per
+ * block of gps_adamw8_block() elements of a chunk (blocks start at the chunk's start; the last may be short).
+ * A block has a unit 2^(E - 127) (E = 0: all zero, 255: not finite) and codes of three mantissa bits: magnitude c stands for c
+ * units below 8 and for (8 + c % 8) * 2^(c / 8 - 1) units from there.  exp_avg: bit 7 is the sign, c < 128; exp_avg_sq: c < 256.
+ * The unit is the smallest power of two that keeps the block's largest magnitude representable (at least 2^-126).
+ * Codes are rounded up or down at random with the probabilities that keep the mean (a moving average that rounds to nearest never
+ * takes a step smaller than half a code); a value of exp_avg_sq that is not zero is not rounded to zero.  The random bits of an
+ * element are mix(index + mix(step * 0x9E3779B9 + seed)), low 16 for exp_avg and high 16 for exp_avg_sq: index = its arena
+ * offset, step = its parameter's step, mix(x): x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16:
+ * the same run gives the same codes.
+ *   m, v           uint8, the arena's layout;  m_exp, v_exp: uint8 [n_chunks * gps_optim_chunk() / gps_adamw8_block()]
+ *   ws             gps_adamw8_workspace_floats(n_chunks) floats; everything else as in gps_adamw_step
+ * The parameter update uses the moments before they are rounded. */
+int gps_adamw8_block(void);
+size_t gps_adamw8_workspace_floats(int64_t n_chunks);
+int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, const int64_t* chunk_off,
+                    const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active, int64_t n_chunks, double* hyper,
+                    float* pstep, uint32_t seed, float* ws, gps_stream_t stream);
+/* The moments' values, arena layout, GPS_F32 or GPS_BF16 (which holds each exactly: four significant bits).  n_gaps pieces
+ * (gap_off, gap_len <= gps_optim_chunk()) that belong to no parameter are set to zero.  Either output may be NULL. */
+int gps_adamw8_values(const uint8_t* m, const uint8_t* v, const uint8_t* m_exp, const uint8_t* v_exp, const int64_t* chunk_off,
+                      const int32_t* chunk_len, int64_t n_chunks, const int64_t* gap_off, const int32_t* gap_len, int64_t n_gaps,
+                      int dtype, void* m_out, void* v_out, gps_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
