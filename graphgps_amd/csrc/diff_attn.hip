@@ -184,7 +184,9 @@ void launch_fwd(const Args& a, hipStream_t s) {
 
 template <typename T>
 void forward(const Args& a, hipStream_t s) {
-  if (a.d <= 32)
+  if (few_applies(a))
+    forward_few<T>(a, s);
+  else if (a.d <= 32)
     launch_fwd<T, 32, 2>(a, s);
   else if (a.d <= 64)
     launch_fwd<T, 64, 2>(a, s);
@@ -211,7 +213,7 @@ int check(const char* who, const Args* a) {
   GPS_REQUIRE(a->q_ptr && a->k_ptr && a->lam, "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nq == 0 || (a->q && a->o), "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nk == 0 || (a->k && a->v), "%s: null pointer argument", who);
-  GPS_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->o2), "%s: pointers must be 16-byte aligned", who);
+  GPS_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->o2) && aligned16(a->ws), "%s: pointers must be 16-byte aligned", who);
   GPS_REQUIRE(by8({a->q_rs, a->q_hs, a->q_ms, a->k_rs, a->k_hs, a->k_ms, a->v_rs, a->v_hs}), "%s: strides must be multiples of 8 elements", who);
   GPS_REQUIRE((a->o2 == nullptr) == (a->lse == nullptr), "%s: o2 and lse come together", who);
   return GPS_OK;
@@ -221,9 +223,16 @@ int check(const char* who, const Args* a) {
 
 extern "C" {
 
+size_t gps_diff_attn_fwd_workspace_floats(const gps_diff_attn* a) {
+  if (!a || a->H <= 0 || a->Hk <= 0 || a->Nq <= 0 || !few_applies(*a)) return 0;
+  return few_workspace_floats(*a);
+}
+
 int gps_diff_attn_fwd(const gps_diff_attn* a, gps_stream_t stream) {
   if (const int rc = check("gps_diff_attn_fwd", a)) return rc;
   if (a->Nq == 0) return GPS_OK;
+  const size_t need = gps_diff_attn_fwd_workspace_floats(a);
+  GPS_REQUIRE(need == 0 || (a->ws && a->ws_floats >= need), "gps_diff_attn_fwd: workspace of %zu floats, %zu needed", a->ws_floats, need);
   hipStream_t s = gps::as_stream(stream);
   if (a->dtype == GPS_F32)
     forward<float>(*a, s);

@@ -135,25 +135,31 @@ __device__ __forceinline__ int clamp_row(int32_t r, int64_t n) { return r < 0 ? 
 // numbers from ptr[s] / bm + s on: that grows by at least ceil(length / bm) from each segment to the next and never passes
 // N / bm + B, so N / bm + B + 1 tiles cover every segment and the rows behind the last one (segment B).  64 lanes probe at a
 // time: two rounds for up to 4,096 segments.  Lane-uniform.  Entries outside [0, N] are cut to it: no row index leaves N.
+template <typename In>
+__device__ __forceinline__ int last_segment(int B, In in) {   // the last s in 0 .. B with in(s); in(0) holds, and in() only ends once
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = B;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) >> 6;
+    const int s = lo + (lane + 1) * step;
+    const int n = __popcll(__ballot(s <= hi && in(s)));
+    lo += n * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+__device__ __forceinline__ int find_segment(const int32_t* ptr, int B, int64_t N, int64_t row) {
+  return last_segment(B, [&](int s) { return clamp_row(ptr[s], N) <= row; });
+}
+
 struct Tile {
   int seg, first, rows;  // segment (B = behind the last one), first row, rows in this tile (<= 0: none)
   int local;             // index of `first` in the segment
   int len;               // rows of the segment
 };
 __device__ __forceinline__ Tile find_tile(const int32_t* ptr, int B, int64_t N, int bm, int tile) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = B;
-  while (lo < hi) {
-    const int step = (hi - lo + 63) >> 6;
-    const int s = lo + (lane + 1) * step;
-    bool in = false;
-    if (s <= hi) in = clamp_row(ptr[s], N) / bm + s <= tile;
-    const int n = __popcll(__ballot(in));
-    lo += n * step;
-    hi = min(hi, lo + step - 1);
-  }
   Tile t;
-  t.seg = __builtin_amdgcn_readfirstlane(lo);
+  t.seg = last_segment(B, [&](int s) { return clamp_row(ptr[s], N) / bm + s <= tile; });
   const int begin = clamp_row(ptr[t.seg], N);
   const int end = t.seg < B ? clamp_row(ptr[t.seg + 1], N) : (int)N;
   t.local = (tile - (begin / bm + t.seg)) * bm;
@@ -179,5 +185,11 @@ __device__ __forceinline__ void stage(T* dst, int ld, const T* src, int64_t row_
 
 template <typename T>
 void backward(const Args& a, hipStream_t s);   // diff_attn_bwd.hip
+
+// diff_attn_few.hip: few queries over many keys
+bool few_applies(const Args& a);
+size_t few_workspace_floats(const Args& a);
+template <typename T>
+void forward_few(const Args& a, hipStream_t s);
 
 }  // namespace diffattn

@@ -333,21 +333,35 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_bwd(Args a) {
   }
 }
 
-// column sums over the workgroups' partial sums: one thread per column and quarter of the partials, quarters in order
-__global__ __launch_bounds__(256) void k_sandwich_cols(const float* __restrict__ ws, int parts, int D, float* o0, float* o1, float* o2,
-                                                       float* o3, float* o4) {
-  __shared__ float sh[4][64];
+// column sums over the workgroups' partial sums: 64 columns x 16 slices of the partials per workgroup, eight loads in flight per
+// thread (a slice of 64 dependent additions is latency, not bandwidth); slices meet in LDS, in order
+__global__ __launch_bounds__(1024) void k_sandwich_cols(const float* __restrict__ ws, int parts, int D, float* o0, float* o1, float* o2,
+                                                        float* o3, float* o4) {
+  __shared__ float sh[16][64];
   float* outs[kSums] = {o0, o1, o2, o3, o4};
   float* out = outs[blockIdx.y];
   if (!out) return;
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), quarter = threadIdx.x >> 6;
-  const float* p = ws + (int64_t)blockIdx.y * parts * D;
+  const int x = threadIdx.x & 63, slice = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
+  const int per = (parts + 15) / 16, i0 = slice * per, i1 = min(parts, i0 + per);
+  const float* p = ws + (int64_t)blockIdx.y * parts * D + min(c, D - 1);
   float s = 0.f;
-  if (c < D)
-    for (int i = quarter; i < parts; i += 4) s += p[(int64_t)i * D + c];
-  sh[quarter][threadIdx.x & 63] = s;
+  int i = i0;
+  for (; i + 8 <= i1; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[(int64_t)(i + j) * D];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += v[j];
+  }
+  for (; i < i1; ++i) s += p[(int64_t)i * D];
+  sh[slice][x] = s;
   __syncthreads();
-  if (quarter == 0 && c < D) out[c] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+  if (slice == 0 && c < D) {
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s += sh[j][x];
+    out[c] = s;
+  }
 }
 
 int64_t rows_per_block(int tpr) { return kThreads / tpr; }
@@ -364,7 +378,7 @@ void launch(const Args& a, bool backward, hipStream_t s) {
   }
   const int blocks = blocks_for(a.N, TPR);
   if (blocks > 0) k_sandwich_bwd<T, TPR, V, NC><<<blocks, kThreads, 0, s>>>(a);
-  k_sandwich_cols<<<dim3((a.D + 63) / 64, kSums), 256, 0, s>>>(a.ws, blocks, a.D, a.dpost_weight, a.dpost_bias, a.dpre_weight,
+  k_sandwich_cols<<<dim3((a.D + 63) / 64, kSums), 1024, 0, s>>>(a.ws, blocks, a.D, a.dpost_weight, a.dpost_bias, a.dpre_weight,
                                                                a.dpre_bias, a.dgate);
 }
 

@@ -112,8 +112,12 @@ class _Call:
             lse = torch.empty(2, self.H, n, dtype=torch.float32, device=dev)
         a = self.block(q, k, v, lam)
         a.o, a.o2, a.lse = ptr(o), ptr(o2), ptr(lse)
+        L = _lib.load()
+        a.ws_floats = L.gps_diff_attn_fwd_workspace_floats(ctypes.addressof(a))
+        ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev) if a.ws_floats else None
+        a.ws = ptr(ws)
         with on_device(dev):
-            check(_lib.load().gps_diff_attn_fwd(ctypes.addressof(a), current_stream(dev)), "gps_diff_attn_fwd")
+            check(L.gps_diff_attn_fwd(ctypes.addressof(a), current_stream(dev)), "gps_diff_attn_fwd")
         return o, o2, lse
 
     def backward(self, q, k, v, lam, o, o2, lse, do, dq, dk, dv):

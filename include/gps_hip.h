@@ -739,7 +739,8 @@ int gps_adamw_step(float* p, const float* g, float* m, float* v, const int64_t* 
  * row / head / map strides multiples of 8 elements.  max_q / max_k: the longest segment if the host knows it, else 0; they choose
  * the launch shape only.
  * Training keeps o2 [Nq, H, 2d] (fp32, the second map's share of o) and lse [2, H, Nq] (fp32); both NULL at inference.
- * Backward workspace: gps_diff_attn_bwd_workspace_floats().  The results do not depend on how work is split: no atomics. */
+ * ws: gps_diff_attn_fwd_workspace_floats() floats of the same argument block (0 unless max_q says that there are few queries: then
+ * the keys are split and joined), gps_diff_attn_bwd_workspace_floats() in the backward; 16-byte aligned.  The results do not depend on how work is split: no atomics. */
 #define GPS_F32 0
 #define GPS_BF16 1
 #define GPS_F16 2
@@ -763,6 +764,7 @@ typedef struct gps_diff_attn {
   size_t ws_floats;
 } gps_diff_attn;
 
+size_t gps_diff_attn_fwd_workspace_floats(const gps_diff_attn* a);
 size_t gps_diff_attn_bwd_workspace_floats(int64_t Nq, int H);
 int gps_diff_attn_fwd(const gps_diff_attn* a, gps_stream_t stream);
 int gps_diff_attn_bwd(const gps_diff_attn* a, gps_stream_t stream);

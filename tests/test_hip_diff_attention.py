@@ -127,6 +127,15 @@ def test_launch_shapes_agree(dtype, hint, lens):
     compare(run(q, k, v, lam, qp, kp, do, max_q=hint, max_k=hint), (q, k, v, lam, qp, kp), do, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("lens,hint", [("mixed", 1), ("long", 2), ("molecules", 3)])
+def test_more_queries_than_the_few_that_were_said(dtype, lens, hint):
+    q, k, v, lam, qp, kp, do = make(LENS[lens], LENS[lens], 4, 2, 40, dtype, seed=16)
+    keep = (torch.rand(k.shape[0], generator=torch.Generator().manual_seed(17)) < 0.8).cuda()
+    got = run(q, k, v, lam, qp, kp, do, max_q=hint, causal=True, key_mask=keep)
+    compare(got, (q, k, v, lam, qp, kp), do, dtype, causal=True, keep=keep)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("q_lens,k_lens", [([40, 3, 0, 70], [40, 9, 5, 200]), ([33, 100, 4], [7, 100, 0]), ([1, 1], [300, 1])])
 @pytest.mark.parametrize("causal", [False, True])
