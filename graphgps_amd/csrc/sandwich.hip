@@ -20,10 +20,17 @@ using Args = gps_sandwich_norm;
 
 constexpr int kThreads = 256;
 constexpr int kSums = 5;          // dw1, db1, dw2, db2, dgate
-constexpr int kMaxBlocks = 1024;  // backward workgroups (= partial sums per column)
+constexpr int kCUs = 256;
+constexpr int kMaxBlocks = 1024;  // most backward workgroups (= partial sums per column)
 
 template <typename T, int V>
 struct Chunk {
+  typedef T Raw __attribute__((ext_vector_type(V)));
+  static __device__ __forceinline__ Raw fetch(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ void widen(const Raw& r, float* x) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = (float)r[i];
+  }
   static __device__ __forceinline__ void load(const T* p, float* x) {
     if constexpr (V == 1) {
       x[0] = (float)p[0];
@@ -211,9 +218,36 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_bwd(Args a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[k][c][i] = 0.f;
 
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.N; row += (int64_t)gridDim.x * RPB) {
-    const float m1 = post ? a.stats[row] : 0.f, r1 = post ? a.stats[a.N + row] : 1.f;
-    const float m2 = pre ? a.stats[2 * a.N + row] : 0.f, r2 = pre ? a.stats[3 * a.N + row] : 1.f;
+  // the next row's operands are fetched before this row's are used: between them lie two reductions over the row
+  using C = Chunk<T, V>;
+  struct Row {
+    typename C::Raw a[NC], g[NC], x[NC], dz[NC], dy[NC];
+    float m1, r1, m2, r2;
+  };
+  auto fetch = [&](int64_t row, Row& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * V;
+      if (col >= D) continue;
+      o.a[c] = C::fetch(static_cast<const T*>(a.a) + row * a.a_rs + col);
+      if (a.gate_full) o.g[c] = C::fetch(static_cast<const T*>(a.gate_full) + row * a.g_rs + col);
+      if (pre && a.x) o.x[c] = C::fetch(static_cast<const T*>(a.x) + row * a.x_rs + col);
+      if (pre && a.dz) o.dz[c] = C::fetch(static_cast<const T*>(a.dz) + row * a.dz_rs + col);
+      if (a.dy) o.dy[c] = C::fetch(static_cast<const T*>(a.dy) + row * a.dy_rs + col);
+    }
+    o.m1 = post ? a.stats[row] : 0.f;
+    o.r1 = post ? a.stats[a.N + row] : 1.f;
+    o.m2 = pre ? a.stats[2 * a.N + row] : 0.f;
+    o.r2 = pre ? a.stats[3 * a.N + row] : 1.f;
+  };
+  const int64_t stride = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  Row next;
+  if (row < a.N) fetch(row, next);
+  for (; row < a.N; row += stride) {
+    const Row R = next;
+    if (row + stride < a.N) fetch(row + stride, next);
+    const float m1 = R.m1, r1 = R.r1, m2 = R.m2, r2 = R.r2;
     float ah[NC][V], nn[NC][V], gt[NC][V], yh[NC][V], gz[NC][V], t[V], w[V], b[V];
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
@@ -223,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_bwd(Args a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) ah[c][i] = nn[c][i] = yh[c][i] = gz[c][i] = gt[c][i] = 0.f;
       if (!in) continue;
-      Chunk<T, V>::load(static_cast<const T*>(a.a) + row * a.a_rs + col, ah[c]);
+      C::widen(R.a[c], ah[c]);
 #pragma unroll
       for (int i = 0; i < V; ++i) ah[c][i] = (ah[c][i] - m1) * r1;
       load_param<V>(a.post_weight, col, w, 1.f);
@@ -231,14 +265,14 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_bwd(Args a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) nn[c][i] = post ? ah[c][i] * w[i] + b[i] : ah[c][i];
       if (a.gate_full)
-        Chunk<T, V>::load(static_cast<const T*>(a.gate_full) + row * a.g_rs + col, gt[c]);
+        C::widen(R.g[c], gt[c]);
       else
         load_param<V>(a.gate, col, gt[c], 1.f);
       if (pre && a.dz) {
 #pragma unroll
         for (int i = 0; i < V; ++i) t[i] = 0.f;
-        if (a.x) Chunk<T, V>::load(static_cast<const T*>(a.x) + row * a.x_rs + col, t);
-        Chunk<T, V>::load(static_cast<const T*>(a.dz) + row * a.dz_rs + col, gz[c]);
+        if (a.x) C::widen(R.x[c], t);
+        C::widen(R.dz[c], gz[c]);
         load_param<V>(a.pre_weight, col, w, 1.f);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -265,7 +299,7 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_bwd(Args a) {
       float gy[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) gy[i] = 0.f;
-      if (a.dy) Chunk<T, V>::load(static_cast<const T*>(a.dy) + row * a.dy_rs + col, gy);
+      if (a.dy) C::widen(R.dy[c], gy);
       load_param<V>(a.post_weight, col, w, 1.f);
       float o1[V], o2[V];
 #pragma unroll
@@ -376,7 +410,14 @@ void launch(const Args& a, bool backward, hipStream_t s) {
     k_sandwich_fwd<T, TPR, V, NC><<<(unsigned)((a.N + kThreads / TPR - 1) / (kThreads / TPR)), kThreads, 0, s>>>(a);
     return;
   }
-  const int blocks = blocks_for(a.N, TPR);
+  // as many workgroups as are resident at once (a second, partly filled dispatch round would cost a whole row walk), each with an
+  // equal share of the rows
+  static const int resident = [] {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, reinterpret_cast<const void*>(&k_sandwich_bwd<T, TPR, V, NC>), kThreads, 0) != hipSuccess || n < 1) n = 1;
+    return kCUs * n;
+  }();
+  const int most = blocks_for(a.N, TPR), blocks = most < resident ? most : resident;
   if (blocks > 0) k_sandwich_bwd<T, TPR, V, NC><<<blocks, kThreads, 0, s>>>(a);
   k_sandwich_cols<<<dim3((a.D + 63) / 64, kSums), 1024, 0, s>>>(a.ws, blocks, a.D, a.dpost_weight, a.dpost_bias, a.dpre_weight,
                                                                a.dpre_bias, a.dgate);

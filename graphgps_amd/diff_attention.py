@@ -12,22 +12,15 @@ synchronisation, no host read-back, no fallback.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib as _lib
-from .lib import DiffAttn, check, current_stream, ptr
+from .lib import DiffAttn, check, current_stream, on_device, ptr
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # GPS_F32, GPS_BF16, GPS_F16
-
-
-def on_device(dev: torch.device):
-    """Makes ``dev`` the current device for a launch (a stream belongs to its device); free when it is already."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _fail(msg: str):
@@ -104,36 +97,41 @@ class _Call:
         return a
 
     def forward(self, q, k, v, lam, train: bool):
-        dev, n = q.device, q.shape[0]
+        """-> (o, kept): ``kept`` is one fp32 buffer, the second map's share [Nq, H, 2d] and then the log-sums [2, H, Nq]."""
+        dev, n, L = q.device, q.shape[0], _lib.load()
         o = torch.empty(n, self.H, 2 * self.d, dtype=q.dtype, device=dev)
-        o2 = lse = None
+        self.args = a = self.block(q, k, v, lam)
+        a.o = o.data_ptr()
+        kept = None
         if train:
-            o2 = torch.empty(n, self.H, 2 * self.d, dtype=torch.float32, device=dev)
-            lse = torch.empty(2, self.H, n, dtype=torch.float32, device=dev)
-        a = self.block(q, k, v, lam)
-        a.o, a.o2, a.lse = ptr(o), ptr(o2), ptr(lse)
-        L = _lib.load()
+            kept = torch.empty(n * self.H * (2 * self.d + 2), dtype=torch.float32, device=dev)
+            if n:
+                at = kept.data_ptr()
+                a.o2, a.lse = at, at + 4 * n * self.H * 2 * self.d
         a.ws_floats = L.gps_diff_attn_fwd_workspace_floats(ctypes.addressof(a))
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev) if a.ws_floats else None
         a.ws = ptr(ws)
         with on_device(dev):
             check(L.gps_diff_attn_fwd(ctypes.addressof(a), current_stream(dev)), "gps_diff_attn_fwd")
-        return o, o2, lse
+        return o, kept
 
-    def backward(self, q, k, v, lam, o, o2, lse, do, dq, dk, dv):
+    def backward(self, q, lam, do, dq, dk, dv):
+        """``q`` and the forward's other tensors are alive (saved), so the forward's argument block still holds."""
+        if torch.is_grad_enabled():
+            _fail("diff_attention is differentiable once: its backward has no gradient of its own")
         L, dev = _lib.load(), q.device
         if do.dtype != q.dtype:
             _fail(f"diff_attention: gradient of type {do.dtype} for an output of type {q.dtype}")
         do = _chunked(do)
         dlam = torch.empty_like(lam)
-        ws = torch.empty(L.gps_diff_attn_bwd_workspace_floats(q.shape[0], self.H), dtype=torch.float32, device=dev)
-        a = self.block(q, k, v, lam)
-        a.o, a.o2, a.lse, a.dout = ptr(o), ptr(o2), ptr(lse), ptr(do)
-        a.dq, a.dk, a.dv, a.dlam, a.ws, a.ws_floats = ptr(dq), ptr(dk), ptr(dv), ptr(dlam), ptr(ws), ws.numel()
-        a.do_rs, a.do_hs = do.stride()[:2]
-        a.dq_rs, a.dq_hs, a.dq_ms = dq.stride()[:3]
-        a.dk_rs, a.dk_hs, a.dk_ms = dk.stride()[:3]
-        a.dv_rs, a.dv_hs = dv.stride()[:2]
+        a = DiffAttn.from_buffer_copy(self.args)
+        a.ws_floats = L.gps_diff_attn_bwd_workspace_floats(a.Nq, a.H)
+        ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev)
+        a.dout, a.dq, a.dk, a.dv, a.dlam, a.ws = [t.data_ptr() for t in (do, dq, dk, dv, dlam, ws)]
+        a.do_rs, a.do_hs, _ = do.stride()
+        a.dq_rs, a.dq_hs, a.dq_ms, _ = dq.stride()
+        a.dk_rs, a.dk_hs, a.dk_ms, _ = dk.stride()
+        a.dv_rs, a.dv_hs, _ = dv.stride()
         with on_device(dev):
             check(L.gps_diff_attn_bwd(ctypes.addressof(a), current_stream(dev)), "gps_diff_attn_bwd")
         return dlam
@@ -143,25 +141,26 @@ class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, call: _Call, train: bool):
         q, k, v, lam = _chunked(q), _chunked(k), _chunked(v), lam.contiguous()
-        o, o2, lse = call.forward(q, k, v, lam, train)
+        o, kept = call.forward(q, k, v, lam, train)
         if train:
-            ctx.save_for_backward(q, k, v, lam, o, o2, lse)
+            ctx.save_for_backward(q, k, v, lam, o, kept)
             ctx.call = call
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
-        q, k, v, lam, o, o2, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dlam = ctx.call.backward(q, k, v, lam, o, o2, lse, do, dq, dk, dv)
+        q, k, v, lam, _, _ = ctx.saved_tensors
+        dq, dk, dv = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)]
+        dlam = ctx.call.backward(q, lam, do, dq, dk, dv)
         return dq, dk, dv, dlam, None, None
 
 
 def _split(qkv: torch.Tensor, H: int, Hk: int, d: int):
-    n = qkv.shape[0]
-    a, b = 2 * H * d, 2 * (H + Hk) * d
-    return qkv[:, :a].view(n, H, 2, d), qkv[:, a:b].view(n, Hk, 2, d), qkv[:, b:].view(n, Hk, 2 * d)
+    """Views of a packed projection's rows: q [n, H, 2, d] | k [n, Hk, 2, d] | v [n, Hk, 2d]."""
+    n, (s, e), at = qkv.shape[0], qkv.stride(), qkv.storage_offset()
+    return (qkv.as_strided((n, H, 2, d), (s, 2 * d * e, d * e, e), at),
+            qkv.as_strided((n, Hk, 2, d), (s, 2 * d * e, d * e, e), at + 2 * H * d * e),
+            qkv.as_strided((n, Hk, 2 * d), (s, 2 * d * e, e), at + 2 * (H + Hk) * d * e))
 
 
 class _DiffSegmentAttention(torch.autograd.Function):
@@ -170,19 +169,18 @@ class _DiffSegmentAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, lam, call: _Call, train: bool):
         qkv, lam = _chunked(qkv), lam.contiguous()
-        o, o2, lse = call.forward(*_split(qkv, call.H, call.Hk, call.d), lam, train)
+        o, kept = call.forward(*_split(qkv, call.H, call.Hk, call.d), lam, train)
         if train:
-            ctx.save_for_backward(qkv, lam, o, o2, lse)
+            ctx.save_for_backward(qkv, lam, o, kept)
             ctx.call = call
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
-        qkv, lam, o, o2, lse = ctx.saved_tensors
+        qkv, lam, _, _ = ctx.saved_tensors
         c = ctx.call
-        d_qkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        dlam = c.backward(*_split(qkv, c.H, c.Hk, c.d), lam, o, o2, lse, do, *_split(d_qkv, c.H, c.Hk, c.d))
+        d_qkv = torch.empty_like(qkv, memory_format=torch.contiguous_format)
+        dlam = c.backward(qkv, lam, do, *_split(d_qkv, c.H, c.Hk, c.d))
         return d_qkv, dlam, None, None
 
 

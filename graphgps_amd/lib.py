@@ -5,6 +5,7 @@ different HIP runtime than PyTorch's, importing/using the ops raises immediately
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
@@ -286,5 +287,11 @@ def current_stream(device: torch.device) -> Optional[int]:
     return _raw_stream(idx)
 
 
+def on_device(dev: torch.device):
+    """Makes ``dev`` the current device for a launch (a stream belongs to its device); free when it is already."""
+    return _NOTHING if dev.index is None or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_NOTHING = contextlib.nullcontext()
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda idx: torch.cuda.current_stream(idx).cuda_stream)

@@ -28,7 +28,7 @@ import torch
 import torch.nn as nn
 
 from . import lib as _lib
-from .lib import check, current_stream, ptr
+from .lib import check, current_stream, on_device, ptr
 
 _ALIGN = 64          # floats (256 B): start of every storage block in the arena
 
@@ -451,7 +451,7 @@ class FlatAdamW8bit(FlatAdamW):
 
     def _launch_step(self) -> None:
         a = self.arena
-        with torch.cuda.device(a.device):
+        with on_device(a.device):
             check(_lib.load().gps_adamw8_step(ptr(a.flat_p), ptr(a.flat_g), ptr(self.exp_avg), ptr(self.exp_avg_sq),
                                               ptr(self.exp_avg_exp), ptr(self.exp_avg_sq_exp), ptr(a.chunk_off), ptr(a.chunk_len),
                                               ptr(a.chunk_param), ptr(a.active), a.n_chunks, ptr(self.hyper), ptr(self.param_step),
@@ -464,7 +464,7 @@ class FlatAdamW8bit(FlatAdamW):
         a = self.arena
         m = torch.empty(a.flat_p.numel(), dtype=dtype, device=a.device)
         v = torch.empty_like(m)
-        with torch.cuda.device(a.device):
+        with on_device(a.device):
             check(_lib.load().gps_adamw8_values(ptr(self.exp_avg), ptr(self.exp_avg_sq), ptr(self.exp_avg_exp),
                                                 ptr(self.exp_avg_sq_exp), ptr(a.chunk_off), ptr(a.chunk_len), a.n_chunks,
                                                 ptr(self._gap_off), ptr(self._gap_len), self._gap_off.numel(),

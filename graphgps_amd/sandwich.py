@@ -12,11 +12,10 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib as _lib
-from .diff_attention import DTYPES, on_device
-from .lib import SandwichNorm, check, current_stream, ptr
+from .diff_attention import DTYPES
+from .lib import SandwichNorm, check, current_stream, on_device, ptr
 
 KINDS = {"rms": 0, "layer": 1}                    # GPS_NORM_RMS, GPS_NORM_LAYER
 
@@ -29,71 +28,71 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """``[..., D]`` -> ``[N, D]``, contiguous within a row."""
     if t is None:
         return None
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.shape[-1] == 1 or t.stride(1) == 1 else t.contiguous()
 
 
 class _Sandwich(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, post_weight, post_bias, pre_weight, pre_bias, gate, alpha, beta, kind, eps, train):
-        shape, dev = a.shape, a.device
+        dev = a.device
         x2, a2 = _rows(x), _rows(a)
         full = gate is not None and gate.dim() > 1
         g2 = _rows(gate) if full else (None if gate is None else gate.contiguous())
         w = [None if t is None else t.contiguous() for t in (post_weight, post_bias, pre_weight, pre_bias)]
         n, d = a2.shape
-        y = torch.empty(shape, dtype=a.dtype, device=dev)
-        z = torch.empty(shape, dtype=a.dtype, device=dev) if pre_weight is not None else None
+        y = torch.empty_like(a, memory_format=torch.contiguous_format)
+        z = torch.empty_like(y) if pre_weight is not None else None
         stats = torch.empty(4, n, dtype=torch.float32, device=dev) if train and (post_weight is not None or pre_weight is not None) else None
-        ctx.set_materialize_grads(False)
-        ctx.form = (n, d, kind, DTYPES[a.dtype], alpha, beta, eps, full, tuple(shape))
-        b = _Sandwich.block(ctx.form, x2, a2, w, g2)
-        b.y, b.z, b.stats = ptr(y), ptr(z), ptr(stats)
+        b = SandwichNorm(a=a2.data_ptr(), x=ptr(x2), gate_full=ptr(g2) if full else None, gate=None if full else ptr(g2),
+                         a_rs=a2.stride(0), x_rs=x2.stride(0) if x is not None else 0, g_rs=g2.stride(0) if full else 0,
+                         post_weight=ptr(w[0]), post_bias=ptr(w[1]), pre_weight=ptr(w[2]), pre_bias=ptr(w[3]), N=n, D=d, kind=kind,
+                         dtype=DTYPES[a.dtype], alpha=alpha, beta=beta, eps=eps, y=y.data_ptr(), z=ptr(z), stats=ptr(stats))
         with on_device(dev):
             check(_lib.load().gps_sandwich_norm_fwd(ctypes.addressof(b), current_stream(dev)), "gps_sandwich_norm_fwd")
         if train:
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(x2, a2, *w, g2, stats)
-            ctx.gate_shape = None if gate is None else gate.shape
+            ctx.block, ctx.shape, ctx.full = b, a.shape, full     # the block's pointers are those of the saved tensors
         return y, z
 
     @staticmethod
-    def block(form, x, a, w, gate) -> SandwichNorm:
-        n, d, kind, dtype, alpha, beta, eps, full, _ = form
-        return SandwichNorm(a=ptr(a), x=ptr(x), gate_full=ptr(gate) if full else None, gate=None if full else ptr(gate),
-                            a_rs=a.stride(0), x_rs=x.stride(0) if x is not None else 0, g_rs=gate.stride(0) if full else 0,
-                            post_weight=ptr(w[0]), post_bias=ptr(w[1]), pre_weight=ptr(w[2]), pre_bias=ptr(w[3]), N=n, D=d, kind=kind,
-                            dtype=dtype, alpha=alpha, beta=beta, eps=eps)
-
-    @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dz):
+        if torch.is_grad_enabled():
+            _fail("sandwich_norm is differentiable once: its backward has no gradient of its own")
         if dy is None and dz is None:
             return (None,) * 12
-        x, a, *w, gate, stats = ctx.saved_tensors
-        n, d, _, _, _, _, _, full, shape = ctx.form
-        dev, L = a.device, _lib.load()
-        need = ctx.needs_input_grad
+        x, a, w1, b1, w2, b2, gate, _ = ctx.saved_tensors
+        dev, L, need, full = a.device, _lib.load(), ctx.needs_input_grad, ctx.full
         dy, dz = _rows(dy), _rows(dz)
         for t in (dy, dz):
             if t is not None and t.dtype != a.dtype:
                 _fail(f"sandwich_norm: gradient of type {t.dtype} for an output of type {a.dtype}")
-
-        def like(t, wanted):
-            return torch.empty(t.shape, dtype=t.dtype, device=dev) if wanted and t is not None else None
-        dx, da = like(x, need[0]), like(a, True)
-        dw = [like(t, need[2 + i]) for i, t in enumerate(w)]
-        dg = like(gate, need[6])
-        ws = torch.empty(L.gps_sandwich_workspace_floats(n, d), dtype=torch.float32, device=dev)
-        b = _Sandwich.block(ctx.form, x, a, w, gate)
-        b.stats, b.dy, b.dz, b.dx, b.da = ptr(stats), ptr(dy), ptr(dz), ptr(dx), ptr(da)
-        b.dy_rs, b.dz_rs = (t.stride(0) if t is not None else 0 for t in (dy, dz))
-        b.dpost_weight, b.dpost_bias, b.dpre_weight, b.dpre_bias = (ptr(t) for t in dw)
-        b.dgate_full, b.dgate = (ptr(dg), None) if full else (None, ptr(dg))
-        b.ws, b.ws_floats = ptr(ws), ws.numel()
+        b = SandwichNorm.from_buffer_copy(ctx.block)
+        n, d = b.N, b.D
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+        da = torch.empty_like(a, memory_format=torch.contiguous_format)
+        dw = [torch.empty_like(t) if need[i] else None for i, t in ((2, w1), (3, b1), (4, w2), (5, b2))]
+        dg = torch.empty_like(gate, memory_format=torch.contiguous_format) if need[6] else None
+        b.ws_floats = L.gps_sandwich_workspace_floats(n, d)
+        ws = torch.empty(b.ws_floats, dtype=torch.float32, device=dev)
+        b.ws, b.dx, b.da = ws.data_ptr(), ptr(dx), da.data_ptr()
+        if dy is not None:
+            b.dy, b.dy_rs = dy.data_ptr(), dy.stride(0)
+        if dz is not None:
+            b.dz, b.dz_rs = dz.data_ptr(), dz.stride(0)
+        b.dpost_weight, b.dpost_bias, b.dpre_weight, b.dpre_bias = [ptr(t) for t in dw]
+        if full:
+            b.dgate_full = ptr(dg)
+        else:
+            b.dgate = ptr(dg)
         with on_device(dev):
             check(L.gps_sandwich_norm_bwd(ctypes.addressof(b), current_stream(dev)), "gps_sandwich_norm_bwd")
-        return (None if dx is None else dx.view(shape), da.view(shape), *dw,
-                None if dg is None else dg.view(ctx.gate_shape), None, None, None, None, None)
+        if len(ctx.shape) != 2:
+            dx, da = (None if t is None else t.view(ctx.shape) for t in (dx, da))
+            dg = dg.view(ctx.shape) if full and dg is not None else dg
+        return (dx, da, *dw, dg, None, None, None, None, None)
 
 
 def sandwich_norm(x: Optional[torch.Tensor], a: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,

@@ -320,3 +320,12 @@ def test_empty_calls():
     q, k, v, lam, qp, kp, do = make([5, 6], [0, 0], 2, 2, 16, F32)
     got = run(q, k, v, lam, qp, kp, do, max_q=6)
     assert all((t == 0).all() for t in got)
+
+
+def test_no_second_derivative():
+    from graphgps_amd import ops
+    from graphgps_amd.lib import GpsHipError
+    q, k, v, lam, qp, kp, do = make([5], [5], 2, 2, 16, F32)
+    o = ops.diff_attention(q.requires_grad_(True), k, v, lam, qp, kp)
+    with pytest.raises(GpsHipError, match="once"):
+        torch.autograd.grad(o, q, do, create_graph=True)

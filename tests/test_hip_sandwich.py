@@ -190,3 +190,12 @@ def test_same_bits_every_time_captured_and_on_another_stream(d):
         want = run(t, "rms", 0.75, 0.5, 1e-5, dy, dz)
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[1]) and all(torch.equal(got[1][n], want[2][n]) for n in want[2])
+
+
+def test_no_second_derivative():
+    from graphgps_amd import ops
+    from graphgps_amd.lib import GpsHipError
+    t, dy, _ = make(5, 16, F32, "rms", "none")
+    y, _ = ops.sandwich_norm(t["x"].requires_grad_(True), t["a"])
+    with pytest.raises(GpsHipError, match="once"):
+        torch.autograd.grad(y, t["x"], dy, create_graph=True)
