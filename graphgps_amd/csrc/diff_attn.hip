@@ -4,7 +4,9 @@
 // BN rows of K (both maps side by side) and V staged in LDS.  Scores are formed as S^T = K Q^T, so that a query is a lane's
 // column: the running maximum and sum of each map need two cross-lane steps per block, the rescaling of the accumulators is by
 // a per-lane scalar, and the weights feed O^T += V^T P^T from the registers they are in.  The two maps keep statistics and
-// accumulators of their own and meet once, in the epilogue.
+// accumulators of their own and meet once, in the epilogue.  Two blocks of K and V are in LDS: one is read while the next one
+// arrives, straight from memory, behind a single barrier per block.  Two wavefronts per SIMD let one's exponentials run under the
+// other's matrix instructions.
 #include <initializer_list>
 
 #include "diff_attn.hpp"
@@ -12,22 +14,19 @@
 namespace {
 using namespace diffattn;
 
-template <typename T>
-struct Cfg {
-  static constexpr int BN = sizeof(T) == 4 ? 32 : 64;      // keys per block
-  static constexpr int Pad = 16 / sizeof(T);               // row pitch of the LDS tiles: + 16 bytes
-};
+// keys per block: 64 where the registers hold two wavefronts per SIMD with it, else 32
+template <typename T, int DQ>
+constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
-template <typename T, int DQ, int QT>
-__global__ __launch_bounds__(256) void k_diff_fwd(Args a) {
-  constexpr int DV = 2 * DQ, DVT = DV / 16, ST = DQ / 32, BN = Cfg<T>::BN, KT = BN / 16;
-  constexpr int LK = 2 * DQ + Cfg<T>::Pad, LV = DV + Cfg<T>::Pad;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
-  T* lk = reinterpret_cast<T*>(lds_raw);
-  T* lv = lk + BN * LK;
-  int* lkeep = reinterpret_cast<int*>(lv + BN * LV);
+template <typename T, int DQ, int QT, bool Masked>
+__global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_diff_fwd(Args a) {
+  constexpr int DV = 2 * DQ, DVT = DV / 16, ST = DQ / 32, BN = block_keys<T, DQ>(), KT = BN / 16;
+  typedef Tl<T, DV> L;   // rows of K (both maps) and of V have the same width
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
+  T* tiles = reinterpret_cast<T*>(lds_raw);                  // [2][K | V]
+  int* lkeep = reinterpret_cast<int*>(tiles + 4 * BN * DV);  // [2][BN]
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
   const int bm = (blockDim.x >> 6) * 16 * QT, h = blockIdx.y, hk = h / (a.H / a.Hk), dv = 2 * a.d;
   const Tile t = find_tile(a.q_ptr, a.B, a.Nq, bm, blockIdx.x);
   if (t.rows <= 0) return;
@@ -39,6 +38,27 @@ __global__ __launch_bounds__(256) void k_diff_fwd(Args a) {
   }
   const int shift = nk - t.len;   // causal: the query at index i of its segment sees keys <= i + shift
   const int last = a.causal ? min(nk, max(0, t.local + t.rows + shift)) : nk;
+
+  const Stager<T, BN, DV, 2> stage_k(a.k_rs, a.k_ms, a.d);
+  const Stager<T, BN, DV, 1> stage_v(a.v_rs, 0, dv);
+  auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
+    T* lk = tiles + buf * 2 * BN * DV;
+    const int64_t base = (int64_t)k0 + kb;
+    const int n = min(BN, nk - kb);
+    const T* ks = static_cast<const T*>(a.k) + base * a.k_rs + hk * a.k_hs;
+    const T* vs = static_cast<const T*>(a.v) + base * a.v_rs + hk * a.v_hs;
+    if constexpr (Masked) {
+      const uint8_t* keep = a.keep + base;
+      auto ok = [&](int r) { return keep[r] != 0; };
+      stage<T, BN, DV, 2>(lk, ks, a.k_rs, a.k_ms, n, a.d, ok);
+      stage<T, BN, DV, 1>(lk + BN * DV, vs, a.v_rs, 0, n, dv, ok);
+      for (int r = threadIdx.x; r < BN; r += blockDim.x) lkeep[buf * BN + r] = r < n && ok(r);
+    } else {
+      stage_k(lk, ks, a.k_rs, a.k_ms, n, a.d);
+      stage_v(lk + BN * DV, vs, a.v_rs, 0, n, dv);
+    }
+  };
+  if (last > 0) fetch(0, 0);
 
   Frag<T> q[2][QT][ST];
   int64_t row[QT];
@@ -58,113 +78,157 @@ __global__ __launch_bounds__(256) void k_diff_fwd(Args a) {
           q[m][i][s] = frag_load(static_cast<const T*>(a.q) + row[i] * a.q_rs + h * a.q_hs + m * a.q_ms + s * 32 + g * 8);
       }
   }
+  const int all_see = a.causal ? t.local + wave * QT * 16 + shift + 1 : nk;   // keys that every query of this wavefront sees
+  // acc[0] = sum (p1 - mix p2) v and acc[1] = sum p2 v with p_i = 2^(score - ref_i): see `mix` below
   f32x4 acc[2][QT][DVT];
-  float top[2][QT], sum[2][QT];
+  float ref[2][QT], sum[2][QT], mix[QT];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int i = 0; i < QT; ++i) {
+    mix[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-      top[m][i] = -kInf;
+    for (int m = 0; m < 2; ++m) {
+      ref[m][i] = -kLowest;
       sum[m][i] = 0.f;
 #pragma unroll
       for (int c = 0; c < DVT; ++c) acc[m][i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  const float scale2 = a.scale * kLog2e;
+  }
+  const float scale2 = a.scale * kLog2e, lam = load_lam(a, h, static_cast<const T*>(nullptr));
 
-  for (int kb = 0; kb < last; kb += BN) {
-    const int64_t base = (int64_t)k0 + kb;
-    const uint8_t* keep = a.keep ? a.keep + base : nullptr;
-    const int n = min(BN, nk - kb);
-    auto ok = [&](int r) { return !keep || keep[r]; };
-    __syncthreads();
+  int buf = 0;
+  for (int kb = 0; kb < last; kb += BN, buf ^= 1) {
+    tiles_ready();
+    if (kb + BN < last) fetch(kb + BN, buf ^ 1);
+    const T* lk = tiles + buf * 2 * BN * DV;
+    const T* lv = lk + BN * DV;
+    f32x4 s[2][QT][KT];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
-      stage<T, BN, DQ>(lk + m * DQ, LK, static_cast<const T*>(a.k) + base * a.k_rs + hk * a.k_hs + m * a.k_ms, a.k_rs, n, a.d, ok);
-    stage<T, BN, DV>(lv, LV, static_cast<const T*>(a.v) + base * a.v_rs + hk * a.v_hs, a.v_rs, n, dv, ok);
-    for (int r = threadIdx.x; r < BN; r += blockDim.x) lkeep[r] = r < n && ok(r);
-    __syncthreads();
-
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      f32x4 s[QT][KT];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-        for (int i = 0; i < QT; ++i) s[i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < QT; ++i) s[m][i][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
-          const Frag<T> kf = frag_load(lk + (kt * 16 + col) * LK + m * DQ + st * 32 + g * 8);
+          const Frag<T> kf = L::frag(lk, kt * 16 + col, m * DQ + st * 32 + g * 8);
 #pragma unroll
-          for (int i = 0; i < QT; ++i) s[i][kt] = mma(kf, q[m][i][st], s[i][kt]);
+          for (int i = 0; i < QT; ++i) s[m][i][kt] = mma(kf, q[m][i][st], s[m][i][kt]);
         }
       }
+    if (Masked || kb + BN > all_see) {   // (uniform over the wavefront)
 #pragma unroll
-      for (int i = 0; i < QT; ++i) {
-        float hi = -kInf;
+      for (int kt = 0; kt < KT; ++kt) {
+        int4 kp = make_int4(1, 1, 1, 1);
+        if constexpr (Masked) kp = *reinterpret_cast<const int4*>(lkeep + buf * BN + kt * 16 + g * 4);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const int4 kp = *reinterpret_cast<const int4*>(lkeep + kt * 16 + g * 4);
+        for (int i = 0; i < QT; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const bool in = (&kp.x)[r] && kb + kt * 16 + g * 4 + r < seen[i];
-            s[i][kt][r] = in ? s[i][kt][r] * scale2 : -kInf;
-            hi = fmaxf(hi, s[i][kt][r]);
+            s[0][i][kt][r] = in ? s[0][i][kt][r] : -kInf;
+            s[1][i][kt][r] = in ? s[1][i][kt][r] : -kInf;
           }
+      }
+    }
+    // The references move only when a score passes one by more than 2^6: weights stay below 64, far inside every type, and the
+    // accumulators are rescaled a few times per row instead of at every new maximum.
+    float hi[2][QT];   // over this lane's keys
+    bool past = false;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        float x = s[m][i][0][0];
+#pragma unroll
+        for (int j = 1; j + 1 < 4 * KT; j += 2) x = maximum(maximum(x, s[m][i][j / 4][j % 4]), s[m][i][(j + 1) / 4][(j + 1) % 4]);
+        hi[m][i] = maximum(x, s[m][i][KT - 1][3]);
+        past |= __builtin_fmaf(hi[m][i], scale2, -ref[m][i]) > 6.f;
+      }
+    const bool move = __any(past);
+    float f[2][QT];
+    if (move) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          const float now = fmaxf(ref[m][i], over_groups(hi[m][i], [](float u, float v) { return maximum(u, v); }) * scale2);
+          f[m][i] = __builtin_amdgcn_exp2f(ref[m][i] - now);
+          ref[m][i] = now;
+          sum[m][i] *= f[m][i];
         }
-        hi = fmaxf(hi, __shfl_xor(hi, 16));
-        hi = fmaxf(hi, __shfl_xor(hi, 32));
-        const float now = fmaxf(top[m][i], hi);
-        const float ref = now == -kInf ? 0.f : now;
-        const float f = __builtin_amdgcn_exp2f(top[m][i] - ref);
-        top[m][i] = now;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
         float add = 0.f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[i][kt][r] = __builtin_amdgcn_exp2f(s[i][kt][r] - ref);
-            add += s[i][kt][r];
+            s[m][i][kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][i][kt][r], scale2, -ref[m][i]));
+            add += s[m][i][kt][r];
           }
-        sum[m][i] = sum[m][i] * f + add;
-#pragma unroll
-        for (int c = 0; c < DVT; ++c) acc[m][i][c] *= f;
+        sum[m][i] += add;
       }
+    // The maps nearly cancel where they agree.  Rounding p1 and p2 to 16 bits apart would leave both errors on that small
+    // difference, so what is rounded is p1 - mix p2, with mix = lam times the ratio of the sums so far: at the end acc[1] enters
+    // with the little that the ratio has moved since.  Changing mix is exact in the accumulators:
+    // sum (p1 - mix' p2) v = acc[0] + (mix - mix') acc[1].
+    if (move) {
 #pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) {
-        Frag<T> p[QT];
-#pragma unroll
-        for (int i = 0; i < QT; ++i) p[i] = frag_pack<T>(s[i][2 * kk], s[i][2 * kk + 1]);
+      for (int i = 0; i < QT; ++i) {
+        const float l1 = over_groups(sum[0][i], [](float u, float v) { return u + v; });
+        const float l2 = over_groups(sum[1][i], [](float u, float v) { return u + v; });
+        const float to = l2 > 0.f ? lam * l1 * __builtin_amdgcn_rcpf(l2) : 0.f;
+        const float with = mix[i] * f[0][i] - to * f[1][i];
+        mix[i] = to;
 #pragma unroll
         for (int c = 0; c < DVT; ++c) {
-          const Frag<T> vf = frag_tr(lv, LV, kk * 32, c * 16, lane);
-#pragma unroll
-          for (int i = 0; i < QT; ++i) acc[m][i][c] = mma(vf, p[i], acc[m][i][c]);
+          acc[0][i][c] = acc[0][i][c] * f[0][i] + acc[1][i][c] * with;
+          acc[1][i][c] *= f[1][i];
         }
       }
     }
+    Frag<T> p[2][QT][BN / 32];
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+      for (int kk = 0; kk < BN / 32; ++kk) {
+        p[0][i][kk] = frag_pack<T>(s[0][i][2 * kk] - s[1][i][2 * kk] * mix[i], s[0][i][2 * kk + 1] - s[1][i][2 * kk + 1] * mix[i]);
+        p[1][i][kk] = frag_pack<T>(s[1][i][2 * kk], s[1][i][2 * kk + 1]);
+      }
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk)
+#pragma unroll
+      for (int c = 0; c < DVT; ++c) {
+        const Frag<T> vf = L::frag_tr(lv, kk * 32, c * 16, lane);
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          acc[0][i][c] = mma(vf, p[0][i][kk], acc[0][i][c]);
+          acc[1][i][c] = mma(vf, p[1][i][kk], acc[1][i][c]);
+        }
+      }
   }
 
-  const float lam = load_lam(a, h, static_cast<const T*>(nullptr));
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     float inv[2], l2[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float z = sum[m][i];
-      z += __shfl_xor(z, 16);
-      z += __shfl_xor(z, 32);
+      const float z = over_groups(sum[m][i], [](float u, float v) { return u + v; });
       inv[m] = z == 0.f ? 0.f : 1.f / z;
-      l2[m] = z == 0.f ? kInf : top[m][i] + __builtin_amdgcn_logf(z);
+      l2[m] = z == 0.f ? kInf : ref[m][i] + __builtin_amdgcn_logf(z);
     }
     if (row[i] < 0) continue;
     const int64_t at = (row[i] * a.H + h) * dv;
+    const float with = mix[i] * inv[0] - lam * inv[1];
 #pragma unroll
     for (int c = 0; c < DVT; ++c) {
       const int x = c * 16 + g * 4;
       if (x >= dv) continue;
-      const f32x4 second = acc[1][i][c] * inv[1];
-      store4(static_cast<T*>(a.o) + at + x, acc[0][i][c] * inv[0] - second * lam);
-      if (a.o2) store4(a.o2 + at + x, second);
+      store4(static_cast<T*>(a.o) + at + x, acc[0][i][c] * inv[0] + acc[1][i][c] * with);
+      if (a.o2) store4(a.o2 + at + x, acc[1][i][c] * inv[1]);
     }
     if (a.lse && g == 0) {
       a.lse[(int64_t)h * a.Nq + row[i]] = l2[0];
@@ -178,8 +242,11 @@ void launch_fwd(const Args& a, hipStream_t s) {
   const int per_wave = 16 * QT;
   const int waves = a.max_q > 0 && a.max_q <= per_wave ? 1 : a.max_q > 0 && a.max_q <= 2 * per_wave ? 2 : 4;
   const dim3 grid((unsigned)(a.Nq / (waves * per_wave) + a.B + 1), (unsigned)a.H);
-  const size_t lds = Cfg<T>::BN * ((4 * DQ + 2 * Cfg<T>::Pad) * sizeof(T) + sizeof(int));
-  k_diff_fwd<T, DQ, QT><<<grid, waves * 64, lds, s>>>(a);
+  const size_t lds = 2 * block_keys<T, DQ>() * (4 * DQ * sizeof(T) + (a.keep ? sizeof(int) : 0));
+  if (a.keep)
+    k_diff_fwd<T, DQ, QT, true><<<grid, waves * 64, lds, s>>>(a);
+  else
+    k_diff_fwd<T, DQ, QT, false><<<grid, waves * 64, lds, s>>>(a);
 }
 
 template <typename T>
@@ -209,12 +276,19 @@ int check(const char* who, const Args* a) {
   GPS_REQUIRE(a->d > 0 && a->d <= 128 && a->d % 8 == 0, "%s: d=%d is no multiple of 8 up to 128", who, a->d);
   GPS_REQUIRE(a->Nq >= 0 && a->Nk >= 0 && a->Nq < (int64_t(1) << 31) && a->Nk < (int64_t(1) << 31), "%s: Nq=%lld Nk=%lld", who,
               (long long)a->Nq, (long long)a->Nk);
+  // the launch grids: tiles of 16 rows at least, 256 threads at most, below 2^32 threads
+  GPS_REQUIRE((a->Nq / 16 + a->B + 1) * a->H + (a->Nk / 16 + a->B + 1) * a->Hk + a->H < (int64_t(1) << 24), "%s: Nq=%lld Nk=%lld B=%d: more tiles than one launch holds",
+              who, (long long)a->Nq, (long long)a->Nk, a->B);
+  GPS_REQUIRE(a->scale > 0.f && a->scale < kInf, "%s: scale %g is not positive", who, (double)a->scale);
   GPS_REQUIRE(a->max_q >= 0 && a->max_k >= 0, "%s: max_q=%d max_k=%d", who, a->max_q, a->max_k);
   GPS_REQUIRE(a->q_ptr && a->k_ptr && a->lam, "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nq == 0 || (a->q && a->o), "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nk == 0 || (a->k && a->v), "%s: null pointer argument", who);
   GPS_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->o2) && aligned16(a->ws), "%s: pointers must be 16-byte aligned", who);
   GPS_REQUIRE(by8({a->q_rs, a->q_hs, a->q_ms, a->k_rs, a->k_hs, a->k_ms, a->v_rs, a->v_hs}), "%s: strides must be multiples of 8 elements", who);
+  // the lanes' offsets within a block of rows are 32-bit
+  for (int64_t x : {a->q_rs, a->k_rs, a->v_rs, a->do_rs}) GPS_REQUIRE(x >= 0 && x <= (1 << 22), "%s: row stride %lld", who, (long long)x);
+  for (int64_t x : {a->q_ms, a->k_ms}) GPS_REQUIRE(x >= 0 && x <= (1 << 28), "%s: map stride %lld", who, (long long)x);
   GPS_REQUIRE((a->o2 == nullptr) == (a->lse == nullptr), "%s: o2 and lse come together", who);
   return GPS_OK;
 }
@@ -251,7 +325,7 @@ int gps_diff_attn_bwd(const gps_diff_attn* a, gps_stream_t stream) {
   GPS_REQUIRE(aligned16(a->dout) && aligned16(a->dq) && aligned16(a->dk) && aligned16(a->dv) &&
                   by8({a->do_rs, a->do_hs, a->dq_rs, a->dq_hs, a->dq_ms, a->dk_rs, a->dk_hs, a->dk_ms, a->dv_rs, a->dv_hs}),
               "gps_diff_attn_bwd: gradients must be 16-byte aligned, their strides multiples of 8 elements");
-  const size_t need = gps_diff_attn_bwd_workspace_floats(a->Nq, a->H);
+  const size_t need = gps_diff_attn_bwd_workspace_floats(a->Nq, a->H, a->B);
   GPS_REQUIRE(need == 0 || (a->ws && a->ws_floats >= need), "gps_diff_attn_bwd: workspace of %zu floats, %zu needed", a->ws_floats, need);
   hipStream_t s = gps::as_stream(stream);
   if (a->dtype == GPS_F32)

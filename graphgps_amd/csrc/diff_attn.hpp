@@ -25,6 +25,7 @@ using vec_t = T __attribute__((ext_vector_type(N)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLowest = 3.4028234e38f;   // -kLowest: the reference of a row that has seen nothing (finite: -inf scores stay weight 0)
 
 using Args = gps_diff_attn;   // include/gps_hip.h
 
@@ -112,6 +113,17 @@ __device__ __forceinline__ Frag<T> frag_tr(const T* m, int ld, int row0, int col
   return f;
 }
 
+// IEEE maximum (a NaN stays one): one instruction, where fmaxf first makes its operands canonical
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// op over the four lane groups (same lane & 15); every lane gets it
+template <typename Op>
+__device__ __forceinline__ float over_groups(float x, Op op) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // four results -> four contiguous elements of T at p (aligned to four elements)
 template <typename T>
 __device__ __forceinline__ void store4(T* p, f32x4 x) {
@@ -169,18 +181,117 @@ __device__ __forceinline__ Tile find_tile(const int32_t* ptr, int B, int64_t N, 
   return t;
 }
 
-// rows [row0, row0 + n) of `src` (C columns of which `cols` exist, both multiples of 8) -> row-major LDS tile of R rows, stride
-// `ld`; rows past `n` and those that ok(r) refuses, and columns past `cols`, are zero: whatever a dropped row holds, 0 * it is
-// never formed.
-template <typename T, int R, int C, typename Ok>
-__device__ __forceinline__ void stage(T* dst, int ld, const T* src, int64_t row_stride, int n, int cols, Ok ok) {
-  constexpr int kEl = 16 / sizeof(T), kPer = C / kEl;
-  for (int i = threadIdx.x; i < R * kPer; i += blockDim.x) {
-    const int r = i / kPer, c = (i % kPer) * kEl;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < n && c < cols && ok(r)) x = *reinterpret_cast<const uint4*>(src + r * row_stride + c);
-    *reinterpret_cast<uint4*>(dst + r * ld + c) = x;
+// --- LDS tiles: R rows of C elements, no padding, 16-byte chunks of a row permuted by its number (chunk c of row r sits at place
+// c ^ swz(r)).  Loads can then go straight from memory to LDS (a wavefront's load fills 1 KB of consecutive LDS, each lane picking its
+// own address in memory), and both readers below touch every bank equally often.
+template <typename T, int C>
+struct Tl {
+  static constexpr int El = 16 / sizeof(T), CH = C / El, RB = C * sizeof(T);   // elements per chunk, chunks and bytes per row
+  static_assert((CH & (CH - 1)) == 0 && RB >= 64, "power of two rows");
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (RB >= 256)
+      return r & 15;
+    else
+      return (r / (256 / RB)) & (CH - 1);
   }
+  static __device__ __forceinline__ int at(int r, int chunk) { return r * C + ((chunk ^ swz(r)) * El); }
+
+  // A / B fragment: eight elements from column c (a multiple of 8) of row r
+  static __device__ __forceinline__ Frag<T> frag(const T* m, int r, int c) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 4) {
+      f.lo = *reinterpret_cast<const f32x4*>(m + at(r, c / 4));
+      f.hi = *reinterpret_cast<const f32x4*>(m + at(r, c / 4 + 1));
+    } else {
+      f.v = *reinterpret_cast<const vec_t<T, 8>*>(m + at(r, c / 8));
+    }
+    return f;
+  }
+  // A fragment of the transpose: row of A = column col0 + (l & 15), slots = rows row0 .. row0 + 31 in frag_pack's order
+  static __device__ __forceinline__ Frag<T> frag_tr(const T* m, int row0, int col0, int lane) {
+    Frag<T> f;
+    const int g = lane >> 4, i = lane & 15;
+    if constexpr (sizeof(T) == 4) {
+      const int c = col0 + i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = row0 + g * 4 + j;
+        f.lo[j] = m[at(r, c >> 2) + (c & 3)];
+        f.hi[j] = m[at(r + 16, c >> 2) + (c & 3)];
+      }
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+      const int r = row0 + g * 4 + (i >> 2), c = col0 + (i & 3) * 4;
+      T* p = const_cast<T*>(m) + at(r, c >> 3) + (c & 7);   // swz(r + 16) = swz(r)
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 16 * C));
+      f.v = __builtin_bit_cast(vec_t<T, 8>, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return f;
+  }
+};
+
+// R rows into the tile `dst` straight from memory (complete after the next wait for vector memory).  The C columns are Maps
+// equal parts, `map_stride` apart in memory, of which `cols` elements exist each.  Rows at and past n (n >= 1) repeat row n - 1 and
+// columns past `cols` repeat the last chunk: they meet weights or operands that are zero, and bring nothing a real key does not.
+template <typename T, int R, int C, int Maps>
+__device__ __forceinline__ void stage_async(T* dst, const T* src, int64_t row_stride, int64_t map_stride, int n, int cols) {
+  typedef Tl<T, C> L;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  for (int i = wave; i < R * L::CH / 64; i += waves) {
+    const int x = i * 64 + lane, r = x / L::CH, chunk = (x % L::CH) ^ L::swz(r);
+    const int m = chunk / (L::CH / Maps), c = min(chunk % (L::CH / Maps) * L::El, cols - L::El);
+    const T* p = src + (int64_t)min(r, n - 1) * row_stride + (Maps > 1 ? m * map_stride : 0) + c;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                     (__attribute__((address_space(3))) void*)(dst + i * 64 * L::El), 16, 0, 0);
+  }
+}
+// The same for workgroups of 256 threads with the lanes' offsets from a tile's first row worked out once: what is left per block is
+// one uniform address.  Tiles that are not full, and smaller workgroups, go through stage_async.
+template <typename T, int R, int C, int Maps>
+struct Stager {
+  typedef Tl<T, C> L;
+  static constexpr int Loads = R * L::CH / 256;
+  uint32_t off[Loads];
+  __device__ __forceinline__ Stager(int64_t row_stride, int64_t map_stride, int cols) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < Loads; ++j) {
+      const int x = (j * 4 + wave) * 64 + lane, r = x / L::CH, chunk = (x % L::CH) ^ L::swz(r);
+      const int m = chunk / (L::CH / Maps), c = min(chunk % (L::CH / Maps) * L::El, cols - L::El);
+      off[j] = (uint32_t)((r * row_stride + (Maps > 1 ? m * map_stride : 0) + c) * (int64_t)sizeof(T));
+    }
+  }
+  __device__ __forceinline__ void operator()(T* dst, const T* src, int64_t row_stride, int64_t map_stride, int n, int cols) const {
+    if (n == R && blockDim.x == 256) {
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+      for (int j = 0; j < Loads; ++j)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(reinterpret_cast<const char*>(src) + off[j]),
+                                         (__attribute__((address_space(3))) void*)(dst + (j * 4 + wave) * 64 * L::El), 16, 0, 0);
+    } else {
+      stage_async<T, R, C, Maps>(dst, src, row_stride, map_stride, n, cols);
+    }
+  }
+};
+// The same through registers, with zeros for rows past n, rows that ok(r) refuses and columns past `cols`: whatever a dropped row
+// holds, 0 * it is never formed.
+template <typename T, int R, int C, int Maps, typename Ok>
+__device__ __forceinline__ void stage(T* dst, const T* src, int64_t row_stride, int64_t map_stride, int n, int cols, Ok ok) {
+  typedef Tl<T, C> L;
+  for (int x = threadIdx.x; x < R * L::CH; x += blockDim.x) {
+    const int r = x / L::CH, chunk = (x % L::CH) ^ L::swz(r);
+    const int m = chunk / (L::CH / Maps), c = chunk % (L::CH / Maps) * L::El;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < n && c < cols && ok(r)) v = *reinterpret_cast<const uint4*>(src + r * row_stride + m * map_stride + c);
+    *reinterpret_cast<uint4*>(dst + x * L::El) = v;
+  }
+}
+// this wavefront's loads into LDS have arrived, and everybody's have: tiles written before are readable, tiles read before are free
+__device__ __forceinline__ void tiles_ready() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
 }
 
 template <typename T>

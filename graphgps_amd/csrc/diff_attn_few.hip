@@ -44,7 +44,8 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
           q[m][s] = frag_load(static_cast<const T*>(a.q) + (int64_t)(q0 + qi) * a.q_rs + h * a.q_hs + m * a.q_ms + s * 32 + g * 8);
       }
     f32x4 acc[2][DVT];
-    float top[2] = {-kInf, -kInf}, sum[2] = {0.f, 0.f};
+    float top[2] = {-kInf, -kInf}, sum[2] = {0.f, 0.f}, mix = 0.f;
+    const float lam = have ? load_lam(a, h, static_cast<const T*>(nullptr)) : 0.f;
 #pragma unroll
     for (int x = 0; x < DVT; ++x) acc[0][x] = acc[1][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -101,6 +102,7 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
         }
       }
       const int in = min(n, seen - kb);
+      float f[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float hi = -kInf;
@@ -110,26 +112,33 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
           for (int r = 0; r < 4; ++r) {
             const bool see = u * 16 + g * 4 + r < in && !((dropped >> (u * 4 + r)) & 1u);
             s[m][u][r] = see ? s[m][u][r] * scale2 : -kInf;
-            hi = fmaxf(hi, s[m][u][r]);
+            hi = maximum(hi, s[m][u][r]);
           }
-        hi = fmaxf(hi, __shfl_xor(hi, 16));
-        hi = fmaxf(hi, __shfl_xor(hi, 32));
-        const float now = fmaxf(top[m], hi), ref = now == -kInf ? 0.f : now;
-        const float f = __builtin_amdgcn_exp2f(top[m] - ref);
+        hi = over_groups(hi, [](float x, float y) { return maximum(x, y); });
+        const float now = fmaxf(top[m], hi), off = now == -kInf ? 0.f : now;
+        f[m] = __builtin_amdgcn_exp2f(top[m] - off);
         top[m] = now;
         float add = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[m][u][r] = __builtin_amdgcn_exp2f(s[m][u][r] - ref);
+            s[m][u][r] = __builtin_amdgcn_exp2f(s[m][u][r] - off);
             add += s[m][u][r];
           }
-        sum[m] = sum[m] * f + add;
-#pragma unroll
-        for (int x = 0; x < DVT; ++x) acc[m][x] *= f;
+        sum[m] = sum[m] * f[m] + add;
       }
-      const Frag<T> p0 = frag_pack<T>(s[0][0], s[0][1]), p1 = frag_pack<T>(s[1][0], s[1][1]);
+      // as in diff_attn.hip: what is rounded is p1 - mix p2, near the difference that is wanted
+      const float l1 = over_groups(sum[0], [](float x, float y) { return x + y; });
+      const float l2 = over_groups(sum[1], [](float x, float y) { return x + y; });
+      const float to = l2 > 0.f ? lam * l1 * __builtin_amdgcn_rcpf(l2) : 0.f, with = mix * f[0] - to * f[1];
+      mix = to;
+#pragma unroll
+      for (int x = 0; x < DVT; ++x) {
+        acc[0][x] = acc[0][x] * f[0] + acc[1][x] * with;
+        acc[1][x] *= f[1];
+      }
+      const Frag<T> p0 = frag_pack<T>(s[0][0] - s[1][0] * mix, s[0][1] - s[1][1] * mix), p1 = frag_pack<T>(s[1][0], s[1][1]);
 #pragma unroll
       for (int x = 0; x < DVT; ++x) {
         const Frag<T> vf = frag_tr(lv, LV, 0, x * 16, lane);
@@ -140,13 +149,11 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
     float* part = a.ws + (((int64_t)unit * a.Hk + hk) * cap + c) * part_floats(dv);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float z = sum[m];
-      z += __shfl_xor(z, 16);
-      z += __shfl_xor(z, 32);
+      const float z = over_groups(sum[m], [](float x, float y) { return x + y; });
       if (!have) continue;
 #pragma unroll
       for (int x = 0; x < DVT; ++x)
-        if (x * 16 + g * 4 < dv) *reinterpret_cast<f32x4*>(part + m * dv + x * 16 + g * 4) = acc[m][x];
+        if (x * 16 + g * 4 < dv) *reinterpret_cast<f32x4*>(part + m * dv + x * 16 + g * 4) = m ? acc[1][x] : acc[0][x] + acc[1][x] * mix;
       if (g == 0) {
         part[2 * dv + 2 * m] = top[m];
         part[2 * dv + 2 * m + 1] = z;
@@ -273,8 +280,11 @@ int few_unit_keys(const Args& a) {
 int64_t few_units(const Args& a) { return a.Nk / few_unit_keys(a) + a.B + 1; }
 int few_columns(const Args& a) { return a.max_q * (a.H / a.Hk); }
 
-// Few queries: all (query, head of a group) pairs of a segment fit two column blocks, and the keys do not fit one unit
-bool few_applies(const Args& a) { return a.max_q > 0 && few_columns(a) <= 32 && (a.max_k == 0 || a.max_k > 64) && a.Nk > 0; }
+// Few queries: all (query, head of a group) pairs of a segment fit two column blocks, the keys do not fit one unit, and the join's
+// grid of one workgroup per row stays far from the launch limit of 2^32 threads
+bool few_applies(const Args& a) {
+  return a.max_q > 0 && a.max_q <= 32 && few_columns(a) <= 32 && (a.max_k == 0 || a.max_k > 64) && a.Nk > 0 && a.Nq <= (1 << 20);
+}
 size_t few_workspace_floats(const Args& a) { return (size_t)few_units(a) * a.Hk * few_columns(a) * (4 * (size_t)a.d + 4); }
 
 template <typename T>

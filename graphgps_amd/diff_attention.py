@@ -28,8 +28,10 @@ def _fail(msg: str):
 
 
 def _chunked(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels read it: contiguous last dimension, 16-byte aligned chunks of eight elements."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    """``t`` as the kernels read it: contiguous last dimension, 16-byte aligned chunks of eight elements, row and map strides whose
+    multiples fit 32 bits."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in st[:-1]) and st[0] <= 1 << 22 and (len(st) < 4 or st[2] <= 1 << 28):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -72,6 +74,8 @@ class _Call:
     """What forward and backward of one call share."""
 
     def __init__(self, q, k, v, lam, q_ptr, k_ptr, causal, key_mask, scale, max_q, max_k):
+        if scale is not None and not 0.0 < float(scale) < float("inf"):
+            _fail(f"diff_attention: scale {scale} is not positive")
         H, Hk, d = _check_inputs(q, k, v, lam, key_mask)
         dev = q.device
         q_ptr = _check_ptr(q_ptr, "q_ptr", dev)
@@ -125,7 +129,7 @@ class _Call:
         do = _chunked(do)
         dlam = torch.empty_like(lam)
         a = DiffAttn.from_buffer_copy(self.args)
-        a.ws_floats = L.gps_diff_attn_bwd_workspace_floats(a.Nq, a.H)
+        a.ws_floats = L.gps_diff_attn_bwd_workspace_floats(a.Nq, a.H, a.B)
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev)
         a.dout, a.dq, a.dk, a.dv, a.dlam, a.ws = [t.data_ptr() for t in (do, dq, dk, dv, dlam, ws)]
         a.do_rs, a.do_hs, _ = do.stride()
@@ -197,7 +201,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
 
     ``causal``: the query at index i of a segment with n queries and m keys sees the keys up to index ``i + m - n``; a key a
     query does not see has to be finite, as in any product with a zero weight.  ``key_mask [Nk]``: False drops a key for all
-    queries; its rows of ``k`` and ``v`` may hold anything.  ``scale`` defaults to ``d ** -0.5``.  ``max_q`` / ``max_k``: the
+    queries; its rows of ``k`` and ``v`` may hold anything.  ``scale`` (positive) defaults to ``d ** -0.5``.  ``max_q`` / ``max_k``: the
     longest segment where the host knows it; they choose the launch shape only, and one query per segment
     (``max_q = 1``) over long key segments is split along the keys.
 

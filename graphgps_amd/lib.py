@@ -128,7 +128,7 @@ _SIGNATURES = {
     "gps_seg_attn_bias_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, c_int64, c_int64, c_int, c_int,
                                       c_float, c_float, c_uint64, _P, _P, _P]),
     "gps_diff_attn_fwd_workspace_floats": (c_size_t, [_P]),
-    "gps_diff_attn_bwd_workspace_floats": (c_size_t, [c_int64, c_int]),
+    "gps_diff_attn_bwd_workspace_floats": (c_size_t, [c_int64, c_int, c_int]),
     "gps_diff_attn_fwd": (c_int, [_P, _P]),
     "gps_diff_attn_bwd": (c_int, [_P, _P]),
     "gps_sandwich_max_width": (c_int, []),

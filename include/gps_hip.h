@@ -735,8 +735,10 @@ int gps_adamw_step(float* p, const float* g, float* m, float* v, const int64_t* 
  * no key, give o = 0 and gradients of 0.  causal: the query at index i of a segment with n queries and m keys sees the keys
  * 0 .. i + m - n.  keep [Nk] bytes, 0 = dropped key (what its rows of k and v hold is not read); NULL = none dropped.
  * dtype of q, k, v, o and of the gradients: GPS_F32, GPS_BF16 or GPS_F16; sums and softmax statistics are fp32.  lam is fp32
- * (lam_f32 != 0) or of that dtype, and so is its gradient.  d a multiple of 8, at most 128; base pointers 16-byte aligned and
- * row / head / map strides multiples of 8 elements.  max_q / max_k: the longest segment if the host knows it, else 0; they choose
+ * (lam_f32 != 0) or of that dtype, and so is its gradient.  d a multiple of 8, at most 128; scale
+ * positive; base pointers 16-byte aligned and
+ * strides multiples of 8 elements, row
+ * strides up to 2^22 and map strides up to 2^28.  max_q / max_k: the longest segment if the host knows it, else 0; they choose
  * the launch shape only.
  * Training keeps o2 [Nq, H, 2d] (fp32, the second map's share of o) and lse [2, H, Nq] (fp32); both NULL at inference.
  * ws: gps_diff_attn_fwd_workspace_floats() floats of the same argument block (0 unless max_q says that there are few queries: then
@@ -765,7 +767,7 @@ typedef struct gps_diff_attn {
 } gps_diff_attn;
 
 size_t gps_diff_attn_fwd_workspace_floats(const gps_diff_attn* a);
-size_t gps_diff_attn_bwd_workspace_floats(int64_t Nq, int H);
+size_t gps_diff_attn_bwd_workspace_floats(int64_t Nq, int H, int B);
 int gps_diff_attn_fwd(const gps_diff_attn* a, gps_stream_t stream);
 int gps_diff_attn_bwd(const gps_diff_attn* a, gps_stream_t stream);
 

@@ -46,6 +46,9 @@ def test_diff_attention_refuses_masks_and_cpu_tensors():
         ops.diff_attention(*diff_args(), key_mask=torch.ones(5, dtype=torch.bool))
     with pytest.raises(GpsHipError, match="key_mask"):
         ops.diff_attention(*diff_args(), key_mask=torch.ones(6))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(GpsHipError, match="scale"):
+            ops.diff_attention(*diff_args(), scale=scale)
     with pytest.raises(GpsHipError, match="no CPU fallback"):
         ops.diff_attention(*diff_args())
 
@@ -64,7 +67,7 @@ def c_block(**kw):
     (dict(dtype=3), "dtype"), (dict(H=3), "H=3"), (dict(Hk=0), "Hk=0"), (dict(d=20), "d=20"), (dict(d=256), "d=256"), (dict(d=0), "d=0"),
     (dict(Nq=-1), "Nq=-1"), (dict(Nk=1 << 31), "Nk="), (dict(max_q=-1), "max_q"), (dict(q_ptr=None), "null"), (dict(lam=None), "null"),
     (dict(q=None), "null"), (dict(v=None), "null"), (dict(q=4), "aligned"), (dict(k_rs=63), "strides"), (dict(lse=16), "together"),
-    (dict(B=-1), "B=-1")])
+    (dict(B=-1), "B=-1"), (dict(scale=0.0), "scale")])
 def test_diff_attention_c_entry_refuses(kw, text):
     L = lib.load()
     for fn in (L.gps_diff_attn_fwd, L.gps_diff_attn_bwd):
@@ -81,11 +84,11 @@ def test_diff_attention_backward_c_entry_refuses():
     for n in ("o2", "lse", "dout", "dq", "dk", "dv", "dlam"):
         setattr(a, n, at)
     assert L.gps_diff_attn_bwd(ctypes.addressof(a), None) == -1 and "workspace" in L.gps_last_error().decode()
-    a.ws, a.ws_floats = at, L.gps_diff_attn_bwd_workspace_floats(4, 2) - 1
+    a.ws, a.ws_floats = at, L.gps_diff_attn_bwd_workspace_floats(4, 2, 1) - 1
     assert L.gps_diff_attn_bwd(ctypes.addressof(a), None) == -1 and "workspace" in L.gps_last_error().decode()
     a.ws_floats, a.dk_rs = 1 << 20, 12
     assert L.gps_diff_attn_bwd(ctypes.addressof(a), None) == -1 and "multiples" in L.gps_last_error().decode()
-    assert L.gps_diff_attn_bwd_workspace_floats(-1, 2) == 0
+    assert L.gps_diff_attn_bwd_workspace_floats(-1, 2, 1) == 0
 
 
 @pytest.mark.parametrize("kw,text", [
