@@ -19,7 +19,7 @@ template <typename T, int DQ>
 constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
 template <typename T, int DQ, int QT, bool Masked>
-__global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_diff_fwd(Args a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2) : DQ == 32 ? 2 : 1) void k_diff_fwd(Args a, int tile_count) {
   constexpr int DV = 2 * DQ, DVT = DV / 16, ST = DQ / 32, BN = block_keys<T, DQ>(), KT = BN / 16;
   typedef Tl<T, DV> L;   // rows of K (both maps) and of V have the same width
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
@@ -27,8 +27,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_dif
   int* lkeep = reinterpret_cast<int*>(tiles + 4 * BN * DV);  // [2][BN]
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
-  const int bm = (blockDim.x >> 6) * 16 * QT, h = blockIdx.y, hk = h / (a.H / a.Hk), dv = 2 * a.d;
-  const Tile t = find_tile(a.q_ptr, a.B, a.Nq, bm, blockIdx.x);
+  const Unit unit = xcd_unit(blockIdx.x, tile_count, a.H);
+  if (unit.tile >= tile_count || unit.head >= a.H) return;
+  const int bm = (blockDim.x >> 6) * 16 * QT, h = unit.head, hk = h / (a.H / a.Hk), dv = 2 * a.d;
+  const Tile t = find_tile(a.q_ptr, a.B, a.Nq, bm, unit.tile);
   if (t.rows <= 0) return;
 
   int k0 = 0, nk = 0;
@@ -39,6 +41,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_dif
   const int shift = nk - t.len;   // causal: the query at index i of its segment sees keys <= i + shift
   const int last = a.causal ? min(nk, max(0, t.local + t.rows + shift)) : nk;
 
+  const RowShare<BN> share;
+  bool kept = true;   // whether this thread's row of the block that was fetched last is a key
   const Stager<T, BN, DV, 2> stage_k(a.k_rs, a.k_ms, a.d);
   const Stager<T, BN, DV, 1> stage_v(a.v_rs, 0, dv);
   auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
@@ -47,16 +51,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_dif
     const int n = min(BN, nk - kb);
     const T* ks = static_cast<const T*>(a.k) + base * a.k_rs + hk * a.k_hs;
     const T* vs = static_cast<const T*>(a.v) + base * a.v_rs + hk * a.v_hs;
-    if constexpr (Masked) {
-      const uint8_t* keep = a.keep + base;
-      auto ok = [&](int r) { return keep[r] != 0; };
-      stage<T, BN, DV, 2>(lk, ks, a.k_rs, a.k_ms, n, a.d, ok);
-      stage<T, BN, DV, 1>(lk + BN * DV, vs, a.v_rs, 0, n, dv, ok);
-      for (int r = threadIdx.x; r < BN; r += blockDim.x) lkeep[buf * BN + r] = r < n && ok(r);
-    } else {
-      stage_k(lk, ks, a.k_rs, a.k_ms, n, a.d);
-      stage_v(lk + BN * DV, vs, a.v_rs, 0, n, dv);
-    }
+    if constexpr (Masked) kept = share.row < n && a.keep[base + min(share.row, n - 1)];
+    stage_k(lk, ks, a.k_rs, a.k_ms, n, a.d);
+    stage_v(lk + BN * DV, vs, a.v_rs, 0, n, dv);
   };
   if (last > 0) fetch(0, 0);
 
@@ -98,9 +95,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DQ == 32 ? 2 : 1) void k_dif
   int buf = 0;
   for (int kb = 0; kb < last; kb += BN, buf ^= 1) {
     tiles_ready();
-    if (kb + BN < last) fetch(kb + BN, buf ^ 1);
     const T* lk = tiles + buf * 2 * BN * DV;
     const T* lv = lk + BN * DV;
+    if constexpr (Masked) {   // scores of dropped keys are cut below; their rows of V would meet weights of 0
+      if (!kept) share.template zero<T, DV>(const_cast<T*>(lv));
+      if (share.part == 0) lkeep[buf * BN + share.row] = kept;
+      __syncthreads();
+    }
+    if (kb + BN < last) fetch(kb + BN, buf ^ 1);
     f32x4 s[2][QT][KT];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -241,12 +243,13 @@ template <typename T, int DQ, int QT>
 void launch_fwd(const Args& a, hipStream_t s) {
   const int per_wave = 16 * QT;
   const int waves = a.max_q > 0 && a.max_q <= per_wave ? 1 : a.max_q > 0 && a.max_q <= 2 * per_wave ? 2 : 4;
-  const dim3 grid((unsigned)(a.Nq / (waves * per_wave) + a.B + 1), (unsigned)a.H);
+  const int tiles = (int)(a.Nq / (waves * per_wave)) + a.B + 1;
+  const unsigned grid = (unsigned)xcd_grid(tiles * a.H);
   const size_t lds = 2 * block_keys<T, DQ>() * (4 * DQ * sizeof(T) + (a.keep ? sizeof(int) : 0));
   if (a.keep)
-    k_diff_fwd<T, DQ, QT, true><<<grid, waves * 64, lds, s>>>(a);
+    k_diff_fwd<T, DQ, QT, true><<<grid, waves * 64, lds, s>>>(a, tiles);
   else
-    k_diff_fwd<T, DQ, QT, false><<<grid, waves * 64, lds, s>>>(a);
+    k_diff_fwd<T, DQ, QT, false><<<grid, waves * 64, lds, s>>>(a, tiles);
 }
 
 template <typename T>
@@ -256,7 +259,7 @@ void forward(const Args& a, hipStream_t s) {
   else if (a.d <= 32)
     launch_fwd<T, 32, 2>(a, s);
   else if (a.d <= 64)
-    launch_fwd<T, 64, 2>(a, s);
+    launch_fwd<T, 64, 1>(a, s);
   else
     launch_fwd<T, 128, 1>(a, s);
 }

@@ -147,6 +147,20 @@ __device__ __forceinline__ int clamp_row(int32_t r, int64_t n) { return r < 0 ? 
 // numbers from ptr[s] / bm + s on: that grows by at least ceil(length / bm) from each segment to the next and never passes
 // N / bm + B, so N / bm + B + 1 tiles cover every segment and the rows behind the last one (segment B).  64 lanes probe at a
 // time: two rounds for up to 4,096 segments.  Lane-uniform.  Entries outside [0, N] are cut to it: no row index leaves N.
+// Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own: workgroup b of `tiles` x `heads` takes a unit such
+// that an XCD works on as few heads as possible (all tiles of a head read the same rows), with neighbouring tiles spread over the
+// XCDs that share a head (they are unequal where segments are, or under a causal mask).  Grid: xcd_grid(tiles * heads).
+struct Unit {
+  int tile, head;
+};
+__device__ __forceinline__ Unit xcd_unit(int b, int tiles, int heads) {
+  const int x = b & 7, i = b >> 3;
+  if (8 % heads == 0) return {i * (8 / heads) + x / heads, x % heads};
+  if (heads % 8 == 0) return {i % tiles, x + 8 * (i / tiles)};
+  return {b % tiles, b / tiles};
+}
+__host__ __device__ __forceinline__ int xcd_grid(int units) { return (units + 7) / 8 * 8; }
+
 template <typename In>
 __device__ __forceinline__ int last_segment(int B, In in) {   // the last s in 0 .. B with in(s); in(0) holds, and in() only ends once
   const int lane = threadIdx.x & 63;
@@ -275,19 +289,17 @@ struct Stager {
     }
   }
 };
-// The same through registers, with zeros for rows past n, rows that ok(r) refuses and columns past `cols`: whatever a dropped row
-// holds, 0 * it is never formed.
-template <typename T, int R, int C, int Maps, typename Ok>
-__device__ __forceinline__ void stage(T* dst, const T* src, int64_t row_stride, int64_t map_stride, int n, int cols, Ok ok) {
-  typedef Tl<T, C> L;
-  for (int x = threadIdx.x; x < R * L::CH; x += blockDim.x) {
-    const int r = x / L::CH, chunk = (x % L::CH) ^ L::swz(r);
-    const int m = chunk / (L::CH / Maps), c = chunk % (L::CH / Maps) * L::El;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < n && c < cols && ok(r)) v = *reinterpret_cast<const uint4*>(src + r * row_stride + m * map_stride + c);
-    *reinterpret_cast<uint4*>(dst + x * L::El) = v;
+// This thread's row of a tile of R rows, and its part in zeroing it: 0 * NaN is not 0, so rows that the contraction meets with a
+// weight of zero must not hold whatever a dropped row holds.  blockDim.x / R threads (one at least) share a row.
+template <int R>
+struct RowShare {
+  int per, row, part;
+  __device__ __forceinline__ RowShare() : per(blockDim.x / R), row(threadIdx.x / (blockDim.x / R)), part(threadIdx.x % (blockDim.x / R)) {}
+  template <typename T, int C>
+  __device__ __forceinline__ void zero(T* tile) const {
+    for (int c = part; c < Tl<T, C>::CH; c += per) *reinterpret_cast<uint4*>(tile + row * C + c * Tl<T, C>::El) = make_uint4(0, 0, 0, 0);
   }
-}
+};
 // this wavefront's loads into LDS have arrived, and everybody's have: tiles written before are readable, tiles read before are free
 __device__ __forceinline__ void tiles_ready() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -87,6 +87,7 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
   const int shift = t.len - nq;                                       // query i sees keys <= i + shift
   const int first = a.causal ? max(0, t.local - shift) : 0;           // first query that sees a key of this tile
 
+  const RowShare<BQ> share;
   const Stager<T, BQ, DV, 2> stage_q(a.q_rs, a.q_ms, a.d);
   const Stager<T, BQ, DV, 1> stage_o(a.do_rs, 0, dv);
   // block of 32 queries from qb of head h -> tiles and statistics `buf`; rows past the segment repeat its last one, `cut` below
@@ -103,15 +104,8 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
     }
     const T* qs = static_cast<const T*>(a.q) + base * a.q_rs + h * a.q_hs;
     const T* os = static_cast<const T*>(a.dout) + base * a.do_rs + h * a.do_hs;
-    if constexpr (Masked) {   // rows that see no key: their dO may hold anything
-      const float* lse = a.lse + (int64_t)h * a.Nq + base;
-      auto any = [&](int r) { return lse[r] < kInf; };
-      stage<T, BQ, DV, 2>(lq, qs, a.q_rs, a.q_ms, n, a.d, any);
-      stage<T, BQ, DV, 1>(lq + BQ * DV, os, a.do_rs, 0, n, dv, any);
-    } else {
-      stage_q(lq, qs, a.q_rs, a.q_ms, n, a.d);
-      stage_o(lq + BQ * DV, os, a.do_rs, 0, n, dv);
-    }
+    stage_q(lq, qs, a.q_rs, a.q_ms, n, a.d);
+    stage_o(lq + BQ * DV, os, a.do_rs, 0, n, dv);
   };
   if (first < nq) fetch(hk * group, first, 0);
 
@@ -152,6 +146,14 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
    const float lam = load_lam(a, h, static_cast<const T*>(nullptr));
    for (int qb = first; qb < nq; qb += BQ, buf ^= 1) {
     tiles_ready();
+    if constexpr (Masked) {   // a query that sees no key has weights of 0 and may hold anything
+      T* t0 = tiles + buf * 2 * BQ * DV;
+      if (!(lst_all[buf * 4 * BQ + share.row] < kInf)) {
+        share.template zero<T, DV>(t0);
+        share.template zero<T, DV>(t0 + BQ * DV);
+      }
+      __syncthreads();
+    }
     if (qb + BQ < nq)
       fetch(h, qb + BQ, buf ^ 1);
     else if (h + 1 < hk * group + group)
@@ -194,6 +196,7 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
             const bool in = live[i] && q < nq && (!a.causal || key <= q + shift);
             p1 = in ? p1 : 0.f;
             p2 = in ? p2 : 0.f;
+            if (Masked) dp[i][u][r] = in ? dp[i][u][r] : 0.f;
           }
           const float x = dp[i][u][r];
           dp[i][u][r] = p1 - p2;                 // W
@@ -271,6 +274,8 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
   const int last = a.causal ? min(nk, max(0, t.local + t.rows + shift)) : nk;
   const float lam = load_lam(a, h, static_cast<const T*>(nullptr)), scale2 = a.scale * kLog2e;
 
+  const RowShare<BK> share;
+  bool kept = true;   // whether this thread's row of the block that was fetched last is a key
   const Stager<T, BK, DV, 2> stage_k(a.k_rs, a.k_ms, a.d);
   const Stager<T, BK, DV, 1> stage_v(a.v_rs, 0, dv);
   auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
@@ -279,16 +284,9 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
     const int n = min(BK, nk - kb);
     const T* ks = static_cast<const T*>(a.k) + base * a.k_rs + hk * a.k_hs;
     const T* vs = static_cast<const T*>(a.v) + base * a.v_rs + hk * a.v_hs;
-    if constexpr (Masked) {
-      const uint8_t* keep = a.keep + base;
-      auto ok = [&](int r) { return keep[r] != 0; };
-      stage<T, BK, DV, 2>(lk, ks, a.k_rs, a.k_ms, n, a.d, ok);
-      stage<T, BK, DV, 1>(lk + BK * DV, vs, a.v_rs, 0, n, dv, ok);
-      for (int r = threadIdx.x; r < BK; r += blockDim.x) lkeep[buf * BK + r] = r < n && ok(r);
-    } else {
-      stage_k(lk, ks, a.k_rs, a.k_ms, n, a.d);
-      stage_v(lk + BK * DV, vs, a.v_rs, 0, n, dv);
-    }
+    if constexpr (Masked) kept = share.row < n && a.keep[base + min(share.row, n - 1)];
+    stage_k(lk, ks, a.k_rs, a.k_ms, n, a.d);
+    stage_v(lk + BK * DV, vs, a.v_rs, 0, n, dv);
   };
   if (last > 0) fetch(0, 0);
 
@@ -334,9 +332,14 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
   int buf = 0;
   for (int kb = 0; kb < last; kb += BK, buf ^= 1) {
     tiles_ready();
-    if (kb + BK < last) fetch(kb + BK, buf ^ 1);
     const T* lk = tiles + buf * 2 * BK * DV;
     const T* lv = lk + BK * DV;
+    if constexpr (Masked) {   // scores and dP of dropped keys are cut below; their rows of K would meet a dS of 0
+      if (!kept) share.template zero<T, DV>(const_cast<T*>(lk));
+      if (share.part == 0) lkeep[buf * BK + share.row] = kept;
+      __syncthreads();
+    }
+    if (kb + BK < last) fetch(kb + BK, buf ^ 1);
     const bool cut = Masked || kb + BK > all_see;   // (uniform over the wavefront)
 
     f32x4 s[2][QT][2], dp[QT][2];
@@ -370,6 +373,7 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
             const bool in = (&kp.x)[r] && kb + u * 16 + g * 4 + r < seen[i];
             p1 = in ? p1 : 0.f;
             p2 = in ? p2 : 0.f;
+            if (Masked) dp[i][u][r] = in ? dp[i][u][r] : 0.f;
           }
           d2 = __builtin_fmaf(p2, dp[i][u][r], d2);
           s[0][i][u][r] = p1 * (dp[i][u][r] - dl[0][i]);
@@ -413,13 +417,17 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
 // Both in one launch: the workgroups of dK / dV first (they are the longest), then those of dQ, which fill the CUs that the last
 // uneven round of the first kind leaves idle.
 template <typename T, int DQ, int RT, bool Masked>
-__global__ __launch_bounds__(256, DQ == 32 ? 2 : 1) void k_diff_bwd(Args a, const float* __restrict__ delta, float* __restrict__ part,
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && DQ <= 64) || DQ == 32 ? 2 : 1) void k_diff_bwd(Args a, const float* __restrict__ delta, float* __restrict__ part,
                                                                     int k_tiles, int q_tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
-  int b = blockIdx.x;
-  if (b < k_tiles * a.Hk) return dkv<T, DQ, RT, Masked>(a, delta, b % k_tiles, b / k_tiles, lds_raw);
-  b -= k_tiles * a.Hk;
-  dq<T, DQ, RT, Masked>(a, delta, part + b, b % q_tiles, b / q_tiles, lds_raw);
+  const int k_units = xcd_grid(k_tiles * a.Hk), b = blockIdx.x;
+  if (b < k_units) {
+    const Unit u = xcd_unit(b, k_tiles, a.Hk);
+    if (u.tile < k_tiles && u.head < a.Hk) dkv<T, DQ, RT, Masked>(a, delta, u.tile, u.head, lds_raw);
+  } else {
+    const Unit u = xcd_unit(b - k_units, q_tiles, a.H);
+    if (u.tile < q_tiles && u.head < a.H) dq<T, DQ, RT, Masked>(a, delta, part + u.head * q_tiles + u.tile, u.tile, u.head, lds_raw);
+  }
 }
 
 template <typename T, int DQ, int RT>
@@ -429,7 +437,7 @@ int launch_bwd(const Args& a, float* part, hipStream_t s) {
   const bool known = a.max_q > 0 && a.max_k > 0;
   const int waves = known && longest <= per_wave ? 1 : known && longest <= 2 * per_wave ? 2 : 4, bm = waves * per_wave;
   const int k_tiles = a.Nk > 0 ? (int)(a.Nk / bm) + a.B + 1 : 0, q_tiles = a.Nq > 0 ? (int)(a.Nq / bm) + a.B + 1 : 0;
-  const unsigned grid = (unsigned)(k_tiles * a.Hk + q_tiles * a.H);
+  const unsigned grid = (unsigned)(xcd_grid(k_tiles * a.Hk) + xcd_grid(q_tiles * a.H));
   const size_t lds = 2 * 32 * (4 * DQ * sizeof(T) + 4 * sizeof(float)) + 16;
   if (grid == 0) return 0;
   if (a.keep)
@@ -446,7 +454,7 @@ template <typename T>
 void backward(const Args& a, hipStream_t s) {
   float* part = a.ws + (int64_t)2 * a.H * a.Nq;
   if (a.Nq > 0) k_diff_delta<T><<<dim3((unsigned)((a.Nq + kDeltaRows - 1) / kDeltaRows), (unsigned)a.H), 256, 0, s>>>(a, a.ws);
-  const int parts = a.d <= 32 ? launch_bwd<T, 32, 2>(a, part, s) : a.d <= 64 ? launch_bwd<T, 64, 2>(a, part, s) : launch_bwd<T, 128, 1>(a, part, s);
+  const int parts = a.d <= 32 ? launch_bwd<T, 32, 2>(a, part, s) : a.d <= 64 ? launch_bwd<T, 64, 1>(a, part, s) : launch_bwd<T, 128, 1>(a, part, s);
   k_diff_dlam<T><<<(unsigned)a.H, 256, 0, s>>>(part, parts, a.dlam, a.lam_f32);
 }
 
