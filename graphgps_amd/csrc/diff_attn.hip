@@ -19,7 +19,7 @@ template <typename T, int DQ>
 constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
 template <typename T, int DQ, int QT, bool Masked>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2) : DQ == 32 ? 2 : 1) void k_diff_fwd(Args a, int tile_count) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2) : DQ == 32 ? 3 : 1) void k_diff_fwd(Args a, int tile_count) {
   constexpr int DV = 2 * DQ, DVT = DV / 16, ST = DQ / 32, BN = block_keys<T, DQ>(), KT = BN / 16;
   typedef Tl<T, DV> L;   // rows of K (both maps) and of V have the same width
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
@@ -257,7 +257,7 @@ void forward(const Args& a, hipStream_t s) {
   if (few_applies(a))
     forward_few<T>(a, s);
   else if (a.d <= 32)
-    launch_fwd<T, 32, 2>(a, s);
+    launch_fwd<T, 32, 1>(a, s);
   else if (a.d <= 64)
     launch_fwd<T, 64, 1>(a, s);
   else

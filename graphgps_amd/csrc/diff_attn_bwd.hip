@@ -417,7 +417,7 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
 // Both in one launch: the workgroups of dK / dV first (they are the longest), then those of dQ, which fill the CUs that the last
 // uneven round of the first kind leaves idle.
 template <typename T, int DQ, int RT, bool Masked>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && DQ <= 64) || DQ == 32 ? 2 : 1) void k_diff_bwd(Args a, const float* __restrict__ delta, float* __restrict__ part,
+__global__ __launch_bounds__(256, DQ == 32 ? 3 : sizeof(T) == 2 && DQ == 64 ? 2 : 1) void k_diff_bwd(Args a, const float* __restrict__ delta, float* __restrict__ part,
                                                                     int k_tiles, int q_tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
   const int k_units = xcd_grid(k_tiles * a.Hk), b = blockIdx.x;
@@ -454,7 +454,7 @@ template <typename T>
 void backward(const Args& a, hipStream_t s) {
   float* part = a.ws + (int64_t)2 * a.H * a.Nq;
   if (a.Nq > 0) k_diff_delta<T><<<dim3((unsigned)((a.Nq + kDeltaRows - 1) / kDeltaRows), (unsigned)a.H), 256, 0, s>>>(a, a.ws);
-  const int parts = a.d <= 32 ? launch_bwd<T, 32, 2>(a, part, s) : a.d <= 64 ? launch_bwd<T, 64, 1>(a, part, s) : launch_bwd<T, 128, 1>(a, part, s);
+  const int parts = a.d <= 32 ? launch_bwd<T, 32, 1>(a, part, s) : a.d <= 64 ? launch_bwd<T, 64, 1>(a, part, s) : launch_bwd<T, 128, 1>(a, part, s);
   k_diff_dlam<T><<<(unsigned)a.H, 256, 0, s>>>(part, parts, a.dlam, a.lam_f32);
 }
 
