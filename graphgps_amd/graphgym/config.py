@@ -247,7 +247,8 @@ def _defaults() -> Dict[str, Any]:
     # graphormer_config.py:7-23
     d["graphormer"] = dict(num_layers=6, embed_dim=80, num_heads=4, dropout=0.0,
                            attention_dropout=0.0, mlp_dropout=0.0, input_dropout=0.0,
-                           use_graph_token=True)
+                           use_graph_token=True,
+                           sandwich=False)      # GraphormerLayer(sandwich=...): not in the reference
     d["posenc_GraphormerBias"] = dict(enable=False, node_degrees_only=False, dim_pe=0,
                                       num_spatial_types=None, num_in_degrees=None,
                                       num_out_degrees=None)

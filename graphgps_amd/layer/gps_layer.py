@@ -12,6 +12,7 @@ What runs where:
                           reference's to_dense_batch padding, key-padding mask and [mask]
                           un-pad -- 3 host syncs per layer -- do not exist here)
                           or csrc/favor.hip (Performer FAVOR+)
+                          or csrc/diff_attn.hip (DiffTransformer, not in the reference)
   * dense projections / FFN / BatchNorm -> rocBLAS + MIOpen through torch
 There is no CPU fallback: on a CPU tensor the ops raise.
 """
@@ -116,10 +117,16 @@ class GPSLayer(nn.Module):
                     "built in this tree") from e
             self.self_attn = SelfAttention(dim=dim_h, heads=num_heads,
                                            dropout=self.attn_dropout, causal=False)
+        elif global_model_type == 'DiffTransformer':
+            if self.attn_dropout > 0.0:
+                raise NotImplementedError("global_model_type='DiffTransformer' has no dropout on its attention weights: set "
+                                          "gt.attn_dropout to 0.0")
+            from .diff_attention_layer import DiffSelfAttention
+            self.self_attn = DiffSelfAttention(dim_h, num_heads)
         elif global_model_type == 'BigBird':
             raise NotImplementedError(
                 "global_model_type='BigBird' (block-sparse attention) is outside the HIP hot path; "
-                "supported: 'None', 'Transformer', 'BiasedTransformer', 'Performer'")
+                "supported: 'None', 'Transformer', 'BiasedTransformer', 'Performer', 'DiffTransformer'")
         else:
             raise ValueError(f"Unsupported global x-former model: {global_model_type}")
         self.global_model_type = global_model_type
@@ -207,7 +214,7 @@ class GPSLayer(nn.Module):
             elif self.global_model_type == 'BiasedTransformer':
                 # Graphormer-like conditioning, requires `batch.attn_bias` (reference :201-203)
                 h_attn = self._sa_block(h, gi, batch.attn_bias)
-            elif self.global_model_type == 'Performer':
+            elif self.global_model_type in ('Performer', 'DiffTransformer'):
                 h_attn = self.self_attn.forward_segments(h, gi)
             else:
                 raise RuntimeError(f"Unexpected {self.global_model_type}")

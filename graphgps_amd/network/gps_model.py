@@ -33,4 +33,7 @@ class GPSModel(GraphGymNetwork):
             attn_dropout=cfg.gt.attn_dropout, layer_norm=cfg.gt.layer_norm, batch_norm=cfg.gt.batch_norm,
             bigbird_cfg=cfg.gt.bigbird, log_attn_weights=cfg.train.mode == 'log-attn-weights')
         self._stack('layers', lambda: GPSLayer(**layer_kwargs), cfg.gt.layers)
+        if halves[1] == 'DiffTransformer':           # the initial weight of the second map grows with the layer's index
+            for i, layer in enumerate(self.layers):
+                layer.self_attn.set_depth(i)
         self._head(dim_out)

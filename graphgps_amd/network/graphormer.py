@@ -23,6 +23,6 @@ class GraphormerModel(GraphGymNetwork):
         self._stack('layers',
                     lambda: GraphormerLayer(embed_dim=gcfg.embed_dim, num_heads=gcfg.num_heads,
                                             dropout=gcfg.dropout, attention_dropout=gcfg.attention_dropout,
-                                            mlp_dropout=gcfg.mlp_dropout),
+                                            mlp_dropout=gcfg.mlp_dropout, sandwich=gcfg.sandwich),
                     gcfg.num_layers)
         self._head(dim_out)

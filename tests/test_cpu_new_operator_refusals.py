@@ -162,3 +162,27 @@ def test_stored_moments_round_to_nearest():
     assert int(code[0]) == 1 and int(code[2]) == 0                 # what is not zero does not become zero
     code, exp = encode_moment(torch.tensor([1.0, float("nan")]), 18)
     assert int(exp[0]) == 255 and (code == 0).all()
+
+
+def test_layers_and_config():
+    import math
+    import os
+    import graphgps_amd as g
+    from graphgps_amd.layer.diff_attention_layer import DiffSelfAttention
+    from graphgps_amd.layer.gps_layer import GPSLayer
+    from graphgps_amd.layer.graphormer_layer import GraphormerLayer
+    from graphgps_amd.optim import FlatAdamW8bit
+    m = g.create_model(os.path.join(g.CONFIG_DIR, "zinc_gps_diff.yaml"), ["gt.layers", 3], 1, 1)
+    assert [layer.self_attn.depth for layer in m.layers] == [0, 1, 2]
+    assert abs(m.layers[2].self_attn.lam0 - (0.8 - 0.6 * math.exp(-0.6))) < 1e-12
+    opt = g.register.optimizer_dict[g.cfg.optim.optimizer](m.parameters(), 1e-3, 0.01)
+    assert isinstance(opt, FlatAdamW8bit) and opt.state_dict()["state"] == {}
+    with pytest.raises(NotImplementedError, match="attn_dropout"):
+        GPSLayer(64, "None", "DiffTransformer", 4, attn_dropout=0.1)
+    for bad in ((64, 5, None), (40, 4, None), (64, 4, 3), (1024, 2, None)):
+        with pytest.raises(ValueError, match="heads"):
+            DiffSelfAttention(*bad)
+    plain, sandwich = GraphormerLayer(80, 8, 0.0, 0.0, 0.0), GraphormerLayer(80, 8, 0.0, 0.0, 0.0, sandwich=True)
+    assert set(sandwich.state_dict()) - set(plain.state_dict()) == {"attention_gate", "mlp_gate", "attention_post_norm.weight",
+                                                                    "attention_post_norm.bias", "mlp_post_norm.weight",
+                                                                    "mlp_post_norm.bias"}
