@@ -4,7 +4,8 @@
 // against 32 with fp32 moments.  A wavefront owns one quantisation block of 256 elements, four per lane: its new maximum is one
 // cross-lane reduction, nothing is written before it is known, and no block is visited twice.
 //   K1 k_sqnorm8 : per-workgroup sums of g^2 over a bounded number of workgroups (so that K2 can re-add them all); advances the
-//                  step counters
+//                  step counters and works out each parameter's bias corrections (two fp64 powers: in K2 they would cost every
+//                  workgroup their registers)
 //   K2 k_adamw8  : every workgroup adds K1's sums in the same order (fp64) -> clip coefficient, then updates its chunks
 #include "gps_common.hpp"
 
@@ -26,14 +27,20 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 __global__ __launch_bounds__(kThreads) void k_sqnorm8(const float* __restrict__ g, const int64_t* __restrict__ chunk_off,
                                                       const int32_t* __restrict__ chunk_len, const int32_t* __restrict__ chunk_param,
                                                       const uint8_t* __restrict__ active, int64_t n_chunks,
-                                                      double* __restrict__ hyper, float* __restrict__ pstep, float* __restrict__ ws) {
+                                                      double* __restrict__ hyper, float* __restrict__ pstep, float* __restrict__ ws,
+                                                      float2* __restrict__ coef) {
   __shared__ float sh[kWaves];
   if (blockIdx.x == 0 && threadIdx.x == 0) hyper[H_STEP] += 1.0;
   float acc = 0.f;
   for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int prm = chunk_param[c];
     if (!active[prm]) continue;
-    if (threadIdx.x == 0 && (c == 0 || chunk_param[c - 1] != prm)) pstep[prm] += 1.0f;
+    if (threadIdx.x == 0 && (c == 0 || chunk_param[c - 1] != prm)) {
+      const float step = pstep[prm] + 1.0f;
+      pstep[prm] = step;
+      coef[prm] = make_float2((float)(hyper[H_LR] / (1.0 - pow(hyper[H_B1], (double)step))),
+                              (float)(1.0 / sqrt(1.0 - pow(hyper[H_B2], (double)step))));
+    }
     const float* gp = g + chunk_off[c];
     const int len = chunk_len[c];
     const int n4 = (reinterpret_cast<uintptr_t>(gp) & 15) == 0 ? len >> 2 : 0;
@@ -66,17 +73,31 @@ __device__ __forceinline__ uint32_t code_of(float y, uint32_t r) {
 }
 
 struct Coef {
-  float decay, one_m_b1, b2, one_m_b2, step_size, inv_bc2_sqrt, eps, clip;
+  float decay, one_m_b1, b2, one_m_b2, eps, clip;
 };
 
-// one element; m and v leave unrounded.  Each operation rounds on its own (no contraction), so that the codes can be
-// reproduced by any fp32 arithmetic.
-__device__ __forceinline__ void update(float& p, float g, float& m, float& v, const Coef& k) {
+// One element; m and v leave unrounded.  Each operation on them rounds on its own (no contraction), so that the codes can be
+// reproduced by any fp32 arithmetic; the update's square root and quotient are the hardware's (1 ulp each).
+__device__ __forceinline__ void update(float& p, float g, float& m, float& v, const Coef& k, float step_size, float inv_bc2_sqrt) {
 #pragma clang fp contract(off)
   g = g * k.clip;
   m = m + k.one_m_b1 * (g - m);
   v = k.b2 * v + k.one_m_b2 * g * g;
-  p = p * k.decay - k.step_size * (m / (sqrtf(v) * k.inv_bc2_sqrt + k.eps));
+  const bool tiny = v < 0x1p-96f;
+  const float root = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v) * (tiny ? 0x1p-32f : 1.0f);
+  p = p * k.decay - step_size * (m * __builtin_amdgcn_rcpf(root * inv_bc2_sqrt + k.eps));
+}
+
+// maximum over the wavefront: two half swaps and four row rotations, no LDS
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(b[0], b[1]);
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xf, 0xf, false));   // row_ror:8
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x124, 0xf, 0xf, false));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x122, 0xf, 0xf, false));
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x121, 0xf, 0xf, false));
 }
 
 __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, const float* __restrict__ g, uint8_t* __restrict__ m,
@@ -84,10 +105,10 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
                                                      const int64_t* __restrict__ chunk_off, const int32_t* __restrict__ chunk_len,
                                                      const int32_t* __restrict__ chunk_param, const uint8_t* __restrict__ active,
                                                      int64_t n_chunks, double* __restrict__ hyper, const float* __restrict__ pstep,
-                                                     uint32_t seed, const float* __restrict__ ws, int n_ws) {
+                                                     uint32_t seed, const float* __restrict__ ws, int n_ws,
+                                                     const float2* __restrict__ coef) {
   __shared__ double shd[kWaves];
   __shared__ Coef shk;
-  __shared__ float sh_step;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double acc = 0.0;
   for (int i = threadIdx.x; i < n_ws; i += kThreads) acc += (double)ws[i];
@@ -106,30 +127,19 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
     // torch.nn.utils.clip_grad_norm_: max_norm / (total_norm + 1e-6), at most 1
     k.clip = most > 0.f ? fminf(1.0f, most / (norm + 1e-6f)) : 1.0f;
     if (most > 0.f && norm != norm) k.clip = norm;
-    k.step_size = k.inv_bc2_sqrt = 0.f;
     shk = k;
-    sh_step = -1.f;
     if (blockIdx.x == 0) hyper[H_NORM] = (double)norm;
   }
   __syncthreads();
 
+  const Coef k = shk;
   for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int prm = chunk_param[c];
     if (!active[prm]) continue;
-    const float step = pstep[prm];
-    if (step != sh_step) {   // the same for the whole workgroup
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        shk.step_size = (float)(hyper[H_LR] / (1.0 - pow(hyper[H_B1], (double)step)));
-        shk.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(hyper[H_B2], (double)step)));
-        sh_step = step;
-      }
-      __syncthreads();
-    }
-    const Coef k = shk;
+    const float2 bc = coef[prm];
     const int64_t off = chunk_off[c];
     const int len = chunk_len[c];
-    const uint32_t key = mix32((uint32_t)(int64_t)step * 0x9E3779B9u + seed);
+    const uint32_t key = mix32((uint32_t)(int64_t)pstep[prm] * 0x9E3779B9u + seed);
     const bool wide = ((reinterpret_cast<uintptr_t>(p + off) | reinterpret_cast<uintptr_t>(g + off)) & 15) == 0 &&
                       ((reinterpret_cast<uintptr_t>(m + off) | reinterpret_cast<uintptr_t>(v + off)) & 3) == 0;
     for (int b = wave; b * kBlock < len; b += kWaves) {
@@ -162,17 +172,14 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
         const float s = units_of(x & 127u) * um;
         M[i] = x & 128u ? -s : s;
         V[i] = units_of(y) * uv;
-        update(P[i], G[i], M[i], V[i], k);
+        update(P[i], G[i], M[i], V[i], k, bc.x, bc.y);
         if (i < n) {
           tm = max(tm, __float_as_uint(M[i]) & 0x7fffffffu);
           tv = max(tv, __float_as_uint(V[i]) & 0x7fffffffu);
         }
       }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) {
-        tm = max(tm, (uint32_t)__shfl_xor((int)tm, o));
-        tv = max(tv, (uint32_t)__shfl_xor((int)tv, o));
-      }
+      tm = wave_max(tm);
+      tv = wave_max(tv);
       const int em = unit_exponent(tm, 18), ev = unit_exponent(tv, 34);
       const float im = unit_of(254 - (em == 255 ? 0 : em)), iv = unit_of(254 - (ev == 255 ? 0 : ev));   // 2^-k
       cm = cv = 0;
@@ -274,7 +281,7 @@ extern "C" {
 
 int gps_adamw8_block(void) { return kBlock; }
 
-size_t gps_adamw8_workspace_floats(int64_t n_chunks) { return n_chunks > 0 ? (size_t)norm_blocks(n_chunks) : 0; }
+size_t gps_adamw8_workspace_floats(int64_t n_chunks) { return n_chunks > 0 ? (size_t)norm_blocks(n_chunks) + 1 + 2 * (size_t)n_chunks : 0; }
 
 int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, const int64_t* chunk_off,
                     const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active, int64_t n_chunks, double* hyper,
@@ -283,12 +290,14 @@ int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m
   if (n_chunks == 0) return GPS_OK;
   GPS_REQUIRE(p && g && m && v && m_exp && v_exp && chunk_off && chunk_len && chunk_param && active && hyper && pstep && ws,
               "gps_adamw8_step: null pointer argument");
+  GPS_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 7) == 0, "gps_adamw8_step: workspace must be 8-byte aligned");
   GPS_REQUIRE(gps_optim_chunk() == kChunk, "gps_adamw8_step: chunk table of %d elements", gps_optim_chunk());
   hipStream_t s = gps::as_stream(stream);
   const int nb = norm_blocks(n_chunks);
-  k_sqnorm8<<<nb, kThreads, 0, s>>>(g, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, ws);
+  float2* coef = reinterpret_cast<float2*>(ws + ((nb + 1) & ~1));   // per parameter: never more of them than chunks
+  k_sqnorm8<<<nb, kThreads, 0, s>>>(g, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, ws, coef);
   k_adamw8<<<(unsigned)(n_chunks < kStepBlocks ? n_chunks : kStepBlocks), kThreads, 0, s>>>(
-      p, g, m, v, m_exp, v_exp, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, seed, ws, nb);
+      p, g, m, v, m_exp, v_exp, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, seed, ws, nb, coef);
   return gps::launch_status("gps_adamw8_step");
 }
 
