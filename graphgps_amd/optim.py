@@ -370,6 +370,8 @@ class FlatAdamW(torch.optim.Optimizer):
         return {"state": state, "param_groups": [g]}
 
     def load_state_dict(self, sd) -> None:
+        if any(st["exp_avg"].dtype == torch.uint8 for st in sd["state"].values()):
+            raise ValueError("FlatAdamW: the state holds 8-bit moments (FlatAdamW8bit); their codes are no numbers here")
         a = self.arena
         g = sd["param_groups"][0]
         for k, v in g.items():

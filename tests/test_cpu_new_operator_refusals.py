@@ -186,3 +186,13 @@ def test_layers_and_config():
     assert set(sandwich.state_dict()) - set(plain.state_dict()) == {"attention_gate", "mlp_gate", "attention_post_norm.weight",
                                                                     "attention_post_norm.bias", "mlp_post_norm.weight",
                                                                     "mlp_post_norm.bias"}
+
+
+def test_fp32_optimizer_refuses_8_bit_state():
+    from graphgps_amd.optim import FlatAdamW
+    p = torch.nn.Parameter(torch.zeros(5))
+    opt = FlatAdamW([p])
+    sd = opt.state_dict()
+    sd["state"][0] = dict(step=torch.tensor(1.0), exp_avg=torch.zeros(5, dtype=torch.uint8), exp_avg_sq=torch.zeros(5, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="8-bit moments"):
+        opt.load_state_dict(sd)
