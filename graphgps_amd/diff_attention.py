@@ -90,28 +90,26 @@ class _Call:
         self.q_ptr, self.k_ptr = q_ptr, k_ptr
         self.keep = None if key_mask is None else key_mask.contiguous().view(torch.uint8)
 
-    def block(self, q, k, v, lam) -> DiffAttn:
-        a = DiffAttn(q=ptr(q), k=ptr(k), v=ptr(v), lam=ptr(lam), q_ptr=ptr(self.q_ptr), k_ptr=ptr(self.k_ptr), keep=ptr(self.keep),
-                     Nq=q.shape[0], Nk=k.shape[0], B=self.q_ptr.numel() - 1, H=self.H, Hk=self.Hk, d=self.d, causal=int(self.causal),
+    def block(self, q, k, v, lam, o, kept) -> DiffAttn:
+        n = q.shape[0]
+        a = DiffAttn(q=ptr(q), k=ptr(k), v=ptr(v), lam=ptr(lam), o=ptr(o), q_ptr=ptr(self.q_ptr), k_ptr=ptr(self.k_ptr), keep=ptr(self.keep),
+                     Nq=n, Nk=k.shape[0], B=self.q_ptr.numel() - 1, H=self.H, Hk=self.Hk, d=self.d, causal=int(self.causal),
                      lam_f32=int(lam.dtype == torch.float32), dtype=DTYPES[q.dtype], max_q=self.max_q, max_k=self.max_k,
                      scale=self.scale)
         a.q_rs, a.q_hs, a.q_ms = q.stride()[:3]
         a.k_rs, a.k_hs, a.k_ms = k.stride()[:3]
         a.v_rs, a.v_hs = v.stride()[:2]
+        if kept is not None and n:
+            at = kept.data_ptr()
+            a.o2, a.lse = at, at + 4 * n * self.H * 2 * self.d
         return a
 
     def forward(self, q, k, v, lam, train: bool):
         """-> (o, kept): ``kept`` is one fp32 buffer, the second map's share [Nq, H, 2d] and then the log-sums [2, H, Nq]."""
         dev, n, L = q.device, q.shape[0], _lib.load()
         o = torch.empty(n, self.H, 2 * self.d, dtype=q.dtype, device=dev)
-        self.args = a = self.block(q, k, v, lam)
-        a.o = o.data_ptr()
-        kept = None
-        if train:
-            kept = torch.empty(n * self.H * (2 * self.d + 2), dtype=torch.float32, device=dev)
-            if n:
-                at = kept.data_ptr()
-                a.o2, a.lse = at, at + 4 * n * self.H * 2 * self.d
+        kept = torch.empty(n * self.H * (2 * self.d + 2), dtype=torch.float32, device=dev) if train else None
+        self.args = a = self.block(q, k, v, lam, o, kept)
         a.ws_floats = L.gps_diff_attn_fwd_workspace_floats(ctypes.addressof(a))
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev) if a.ws_floats else None
         a.ws = ptr(ws)
@@ -119,16 +117,15 @@ class _Call:
             check(L.gps_diff_attn_fwd(ctypes.addressof(a), current_stream(dev)), "gps_diff_attn_fwd")
         return o, kept
 
-    def backward(self, q, lam, do, dq, dk, dv):
-        """``q`` and the forward's other tensors are alive (saved), so the forward's argument block still holds."""
+    def backward(self, a: DiffAttn, lam, do, dq, dk, dv):
+        """``a``: the inputs' argument block, which is the backward's from here on."""
         if torch.is_grad_enabled():
             _fail("diff_attention is differentiable once: its backward has no gradient of its own")
-        L, dev = _lib.load(), q.device
-        if do.dtype != q.dtype:
-            _fail(f"diff_attention: gradient of type {do.dtype} for an output of type {q.dtype}")
+        L, dev = _lib.load(), dq.device
+        if do.dtype != dq.dtype:
+            _fail(f"diff_attention: gradient of type {do.dtype} for an output of type {dq.dtype}")
         do = _chunked(do)
         dlam = torch.empty_like(lam)
-        a = DiffAttn.from_buffer_copy(self.args)
         a.ws_floats = L.gps_diff_attn_bwd_workspace_floats(a.Nq, a.H, a.B)
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev)
         a.dout, a.dq, a.dk, a.dv, a.dlam, a.ws = [t.data_ptr() for t in (do, dq, dk, dv, dlam, ws)]
@@ -141,6 +138,12 @@ class _Call:
         return dlam
 
 
+def where(*tensors):
+    """What an argument block holds of tensors: while it is the same, so is the block.  Hooks on saved tensors (activation checkpoints,
+    offloading) may hand a backward other memory than its forward had."""
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+
+
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, call: _Call, train: bool):
@@ -148,14 +151,16 @@ class _DiffAttention(torch.autograd.Function):
         o, kept = call.forward(q, k, v, lam, train)
         if train:
             ctx.save_for_backward(q, k, v, lam, o, kept)
-            ctx.call = call
+            ctx.call, ctx.at = call, where(q, k, v, lam, o, kept)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, lam, _, _ = ctx.saved_tensors
+        q, k, v, lam, o, kept = ctx.saved_tensors
         dq, dk, dv = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)]
-        dlam = ctx.call.backward(q, lam, do, dq, dk, dv)
+        c = ctx.call
+        a = DiffAttn.from_buffer_copy(c.args) if where(q, k, v, lam, o, kept) == ctx.at else c.block(q, k, v, lam, o, kept)
+        dlam = c.backward(a, lam, do, dq, dk, dv)
         return dq, dk, dv, dlam, None, None
 
 
@@ -176,15 +181,17 @@ class _DiffSegmentAttention(torch.autograd.Function):
         o, kept = call.forward(*_split(qkv, call.H, call.Hk, call.d), lam, train)
         if train:
             ctx.save_for_backward(qkv, lam, o, kept)
-            ctx.call = call
+            ctx.call, ctx.at = call, where(qkv, lam, o, kept)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        qkv, lam, _, _ = ctx.saved_tensors
+        qkv, lam, o, kept = ctx.saved_tensors
         c = ctx.call
         d_qkv = torch.empty_like(qkv, memory_format=torch.contiguous_format)
-        dlam = c.backward(qkv, lam, do, *_split(d_qkv, c.H, c.Hk, c.d))
+        same = where(qkv, lam, o, kept) == ctx.at
+        a = DiffAttn.from_buffer_copy(c.args) if same else c.block(*_split(qkv, c.H, c.Hk, c.d), lam, o, kept)
+        dlam = c.backward(a, lam, do, *_split(d_qkv, c.H, c.Hk, c.d))
         return d_qkv, dlam, None, None
 
 

@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import lib as _lib
-from .diff_attention import DTYPES
+from .diff_attention import DTYPES, where
 from .lib import SandwichNorm, check, current_stream, on_device, ptr
 
 KINDS = {"rms": 0, "layer": 1}                    # GPS_NORM_RMS, GPS_NORM_LAYER
@@ -33,6 +33,13 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t.shape[-1] == 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _block(x, a, w, gate, full: bool, stats, kind, alpha, beta, eps) -> SandwichNorm:
+    return SandwichNorm(a=a.data_ptr(), x=ptr(x), gate_full=ptr(gate) if full else None, gate=None if full else ptr(gate),
+                        a_rs=a.stride(0), x_rs=x.stride(0) if x is not None else 0, g_rs=gate.stride(0) if full else 0,
+                        post_weight=ptr(w[0]), post_bias=ptr(w[1]), pre_weight=ptr(w[2]), pre_bias=ptr(w[3]), N=a.shape[0],
+                        D=a.shape[1], kind=kind, dtype=DTYPES[a.dtype], alpha=alpha, beta=beta, eps=eps, stats=ptr(stats))
+
+
 class _Sandwich(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, post_weight, post_bias, pre_weight, pre_bias, gate, alpha, beta, kind, eps, train):
@@ -45,16 +52,14 @@ class _Sandwich(torch.autograd.Function):
         y = torch.empty_like(a, memory_format=torch.contiguous_format)
         z = torch.empty_like(y) if pre_weight is not None else None
         stats = torch.empty(4, n, dtype=torch.float32, device=dev) if train and (post_weight is not None or pre_weight is not None) else None
-        b = SandwichNorm(a=a2.data_ptr(), x=ptr(x2), gate_full=ptr(g2) if full else None, gate=None if full else ptr(g2),
-                         a_rs=a2.stride(0), x_rs=x2.stride(0) if x is not None else 0, g_rs=g2.stride(0) if full else 0,
-                         post_weight=ptr(w[0]), post_bias=ptr(w[1]), pre_weight=ptr(w[2]), pre_bias=ptr(w[3]), N=n, D=d, kind=kind,
-                         dtype=DTYPES[a.dtype], alpha=alpha, beta=beta, eps=eps, y=y.data_ptr(), z=ptr(z), stats=ptr(stats))
+        b = _block(x2, a2, w, g2, full, stats, kind, alpha, beta, eps)
+        b.y, b.z = y.data_ptr(), ptr(z)
         with on_device(dev):
             check(_lib.load().gps_sandwich_norm_fwd(ctypes.addressof(b), current_stream(dev)), "gps_sandwich_norm_fwd")
         if train:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(x2, a2, *w, g2, stats)
-            ctx.block, ctx.shape, ctx.full = b, a.shape, full     # the block's pointers are those of the saved tensors
+            ctx.block, ctx.at, ctx.shape, ctx.full = b, where(x2, a2, *w, g2, stats), a.shape, full
         return y, z
 
     @staticmethod
@@ -63,13 +68,15 @@ class _Sandwich(torch.autograd.Function):
             _fail("sandwich_norm is differentiable once: its backward has no gradient of its own")
         if dy is None and dz is None:
             return (None,) * 12
-        x, a, w1, b1, w2, b2, gate, _ = ctx.saved_tensors
+        saved = x, a, w1, b1, w2, b2, gate, stats = ctx.saved_tensors
         dev, L, need, full = a.device, _lib.load(), ctx.needs_input_grad, ctx.full
         dy, dz = _rows(dy), _rows(dz)
         for t in (dy, dz):
             if t is not None and t.dtype != a.dtype:
                 _fail(f"sandwich_norm: gradient of type {t.dtype} for an output of type {a.dtype}")
         b = SandwichNorm.from_buffer_copy(ctx.block)
+        if where(*saved) != ctx.at:
+            b = _block(x, a, (w1, b1, w2, b2), gate, full, stats, b.kind, b.alpha, b.beta, b.eps)
         n, d = b.N, b.D
         dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
         da = torch.empty_like(a, memory_format=torch.contiguous_format)

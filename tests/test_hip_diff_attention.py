@@ -329,3 +329,54 @@ def test_no_second_derivative():
     o = ops.diff_attention(q.requires_grad_(True), k, v, lam, qp, kp)
     with pytest.raises(GpsHipError, match="once"):
         torch.autograd.grad(o, q, do, create_graph=True)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "offload"])
+@pytest.mark.parametrize("max_q", [0, 2])
+def test_saved_tensors_that_come_back_elsewhere(how, max_q):
+    """Activation checkpoints compute them anew and offloading copies them (contiguous): the gradients stay the same bits."""
+    from graphgps_amd import ops
+    q, k, v, lam, qp, kp, do = make([2, 1, 2], [200, 90, 131], 4, 2, 40, F32, seed=5)
+    want = run(q, k, v, lam, qp, kp, do, max_q=max_q)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+
+    def call(q, k, v, lam):
+        # inputs that live in the graph only: sliced out of wider rows, so their strides are not those of a copy
+        q, v = torch.cat([q * 1.0, q], 1)[:, :4], torch.cat([v * 1.0, v], 1)[:, :2]
+        return ops.diff_attention(q, k * 1.0, v, lam * 1.0, qp, kp, max_q=max_q)
+    if how == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+        o = checkpoint(call, *leaves, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            o = call(*leaves)
+    junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]   # takes what the forward freed
+    got = [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    del junk
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "offload"])
+def test_packed_projection_that_comes_back_elsewhere(how):
+    from graphgps_amd import ops
+    lens, H, d = LENS["molecules"], 4, 24
+    q, k, v, lam, qp, _, do = make(lens, lens, H, H, d, BF16, seed=8)
+    n = q.shape[0]
+    gi = ops.build_graph_index(torch.zeros(2, 0, dtype=torch.int64, device="cuda"), n, len(lens), ptr_vec=qp)
+    gi.nmax_host = max(lens)
+    qkv, lam = torch.cat([t.reshape(n, -1) for t in (q, k, v)], 1).requires_grad_(True), lam.requires_grad_(True)
+    want = torch.autograd.grad(ops.diff_segment_attention(qkv, lam, gi, H), [qkv, lam], do)
+
+    def call(qkv, lam):
+        return ops.diff_segment_attention(torch.cat([qkv, qkv], 1)[:, :qkv.shape[1]], lam * 1.0, gi, H)
+    if how == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+        o = checkpoint(call, qkv, lam, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            o = call(qkv, lam)
+    junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+    got = torch.autograd.grad(o, [qkv, lam], do)
+    del junk
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

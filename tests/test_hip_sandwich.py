@@ -199,3 +199,30 @@ def test_no_second_derivative():
     y, _ = ops.sandwich_norm(t["x"].requires_grad_(True), t["a"])
     with pytest.raises(GpsHipError, match="once"):
         torch.autograd.grad(y, t["x"], dy, create_graph=True)
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "offload"])
+@pytest.mark.parametrize("gate", ["channel", "full"])
+def test_saved_tensors_that_come_back_elsewhere(how, gate):
+    """Activation checkpoints compute them anew and offloading copies them (contiguous): the gradients stay the same bits."""
+    from graphgps_amd import ops
+    t, dy, dz = make(301, 96, F32, "layer", gate, seed=4)
+    want = run(t, "layer", 0.75, 0.5, 1e-5, dy, dz)[2]
+    leaves = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+
+    def call(x, a, *rest):
+        wide = torch.cat([a * 1.0, a], 1)[:, :a.shape[1]]      # rows whose stride a copy does not keep
+        return ops.sandwich_norm(x * 1.0, wide, residual_scale=0.75, branch_scale=0.5, kind="layer",
+                                 **{n: v * 1.0 for n, v in zip(NAMES[2:], rest)})
+    args = [leaves[n] for n in NAMES]
+    if how == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+        y, z = checkpoint(call, *args, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            y, z = call(*args)
+    junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]
+    got = torch.autograd.grad([y, z], args, [dy, dz])
+    del junk
+    for n, g in zip(NAMES, got):
+        assert torch.equal(g, want[n]), n
