@@ -21,6 +21,7 @@ using Args = gps_sandwich_norm;
 constexpr int kThreads = 256;
 constexpr int kSums = 5;          // dw1, db1, dw2, db2, dgate
 constexpr int kCUs = 256;
+constexpr int kGridX = 1 << 20;   // forward workgroups in one row of the grid (a grid dimension holds fewer than 2^32 threads)
 constexpr int kMaxBlocks = 1024;  // most backward workgroups (= partial sums per column)
 
 template <typename T, int V>
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void k_sandwich_fwd(Args a) {
   __shared__ float sh[2][kThreads / 64][2];
   int turn = 0;
   const int lane = threadIdx.x % TPR, D = a.D;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / TPR;
   if (row >= a.N) return;   // rows of one wavefront may leave here: sums are within the lanes of a row (TPR <= 64) or the
                             // whole workgroup has the same row (TPR = 256)
   const bool layer = a.kind == GPS_NORM_LAYER;
@@ -407,7 +408,9 @@ int blocks_for(int64_t N, int tpr) {
 template <typename T, int TPR, int V, int NC>
 void launch(const Args& a, bool backward, hipStream_t s) {
   if (!backward) {
-    k_sandwich_fwd<T, TPR, V, NC><<<(unsigned)((a.N + kThreads / TPR - 1) / (kThreads / TPR)), kThreads, 0, s>>>(a);
+    const int64_t blocks = (a.N + rows_per_block(TPR) - 1) / rows_per_block(TPR);
+    const unsigned x = (unsigned)(blocks < kGridX ? blocks : kGridX);
+    k_sandwich_fwd<T, TPR, V, NC><<<dim3(x, (unsigned)((blocks + x - 1) / x)), kThreads, 0, s>>>(a);
     return;
   }
   // as many workgroups as are resident at once (a second, partly filled dispatch round would cost a whole row walk), each with an

@@ -226,3 +226,16 @@ def test_saved_tensors_that_come_back_elsewhere(how, gate):
     del junk
     for n, g in zip(NAMES, got):
         assert torch.equal(g, want[n]), n
+
+
+def test_more_rows_than_one_grid_dimension_holds():
+    """2^24 workgroups of 256 threads are 2^32 threads: one row per workgroup at this width, so the grid needs a second dimension."""
+    from graphgps_amd import ops
+    n, d = (1 << 24) + 3, 257
+    a = torch.zeros(n, d, dtype=F16, device="cuda")
+    some = torch.cat([torch.arange(5), (1 << 20) + torch.arange(-2, 3), torch.arange(n - 5, n)]).cuda()
+    a[some] = torch.randn(len(some), d, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
+    w = torch.ones(d, device="cuda")
+    y, _ = ops.sandwich_norm(None, a, post_weight=w)
+    want, _ = ops.sandwich_norm(None, a[some], post_weight=w)
+    assert torch.equal(y[some], want) and int(torch.count_nonzero(want)) > 0
