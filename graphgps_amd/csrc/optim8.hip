@@ -3,10 +3,10 @@
 // HBM-bound: p read and written, g read (twice with the norm), a byte read and written for each moment = 20 B per parameter
 // against 32 with fp32 moments.  A wavefront owns one quantisation block of 256 elements, four per lane: its new maximum is one
 // cross-lane reduction, nothing is written before it is known, and no block is visited twice.
-//   K1 k_sqnorm8 : per-workgroup sums of g^2 over a bounded number of workgroups (so that K2 can re-add them all); advances the
-//                  step counters and works out each parameter's bias corrections (two fp64 powers: in K2 they would cost every
-//                  workgroup their registers)
-//   K2 k_adamw8  : every workgroup adds K1's sums in the same order (fp64) -> clip coefficient, then updates its chunks
+//   K1 k_sqnorm8 : per-workgroup sums of g^2 over a bounded number of workgroups (so that K2 can re-add them all); works out each
+//                  chunk's bias corrections (two fp64 powers: in K2 they would cost every workgroup their registers)
+//   K2 k_adamw8  : every workgroup adds K1's sums in the same order (fp64) -> clip coefficient, then updates its chunks; a
+//                  parameter's first chunk advances its step counter
 #include "gps_common.hpp"
 
 namespace {
@@ -19,6 +19,10 @@ constexpr int kNormBlocks = 1024, kStepBlocks = 2048;
 
 enum { H_LR = 0, H_B1, H_B2, H_EPS, H_WD, H_MAXNORM, H_STEP, H_NORM, H_COUNT };
 
+struct ChunkCoef {   // one chunk's step number (its parameter's) and bias corrections
+  float step, size, inv_bc2_sqrt;
+};
+
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   x ^= x >> 16; x *= 0x7feb352dU; x ^= x >> 15; x *= 0x846ca68bU; x ^= x >> 16;
   return x;
@@ -27,19 +31,24 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 __global__ __launch_bounds__(kThreads) void k_sqnorm8(const float* __restrict__ g, const int64_t* __restrict__ chunk_off,
                                                       const int32_t* __restrict__ chunk_len, const int32_t* __restrict__ chunk_param,
                                                       const uint8_t* __restrict__ active, int64_t n_chunks,
-                                                      double* __restrict__ hyper, float* __restrict__ pstep, float* __restrict__ ws,
-                                                      float2* __restrict__ coef) {
+                                                      double* __restrict__ hyper, const float* __restrict__ pstep,
+                                                      float* __restrict__ ws, ChunkCoef* __restrict__ coef) {
   __shared__ float sh[kWaves];
+  int known = -1;   // the parameter that `mine` is of (thread 0)
+  ChunkCoef mine = {};
   if (blockIdx.x == 0 && threadIdx.x == 0) hyper[H_STEP] += 1.0;
   float acc = 0.f;
   for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int prm = chunk_param[c];
     if (!active[prm]) continue;
-    if (threadIdx.x == 0 && (c == 0 || chunk_param[c - 1] != prm)) {
-      const float step = pstep[prm] + 1.0f;
-      pstep[prm] = step;
-      coef[prm] = make_float2((float)(hyper[H_LR] / (1.0 - pow(hyper[H_B1], (double)step))),
-                              (float)(1.0 / sqrt(1.0 - pow(hyper[H_B2], (double)step))));
+    if (threadIdx.x == 0) {
+      if (prm != known) {
+        known = prm;
+        mine.step = pstep[prm] + 1.0f;
+        mine.size = (float)(hyper[H_LR] / (1.0 - pow(hyper[H_B1], (double)mine.step)));
+        mine.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(hyper[H_B2], (double)mine.step)));
+      }
+      coef[c] = mine;
     }
     const float* gp = g + chunk_off[c];
     const int len = chunk_len[c];
@@ -104,9 +113,9 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
                                                      uint8_t* __restrict__ v, uint8_t* __restrict__ m_exp, uint8_t* __restrict__ v_exp,
                                                      const int64_t* __restrict__ chunk_off, const int32_t* __restrict__ chunk_len,
                                                      const int32_t* __restrict__ chunk_param, const uint8_t* __restrict__ active,
-                                                     int64_t n_chunks, double* __restrict__ hyper, const float* __restrict__ pstep,
+                                                     int64_t n_chunks, double* __restrict__ hyper, float* __restrict__ pstep,
                                                      uint32_t seed, const float* __restrict__ ws, int n_ws,
-                                                     const float2* __restrict__ coef) {
+                                                     const ChunkCoef* __restrict__ coef) {
   __shared__ double shd[kWaves];
   __shared__ Coef shk;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -136,10 +145,11 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
   for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int prm = chunk_param[c];
     if (!active[prm]) continue;
-    const float2 bc = coef[prm];
+    const ChunkCoef bc = coef[c];
+    if (threadIdx.x == 0 && (c == 0 || chunk_param[c - 1] != prm)) pstep[prm] = bc.step;
     const int64_t off = chunk_off[c];
     const int len = chunk_len[c];
-    const uint32_t key = mix32((uint32_t)(int64_t)pstep[prm] * 0x9E3779B9u + seed);
+    const uint32_t key = mix32((uint32_t)(int64_t)bc.step * 0x9E3779B9u + seed);
     const bool wide = ((reinterpret_cast<uintptr_t>(p + off) | reinterpret_cast<uintptr_t>(g + off)) & 15) == 0 &&
                       ((reinterpret_cast<uintptr_t>(m + off) | reinterpret_cast<uintptr_t>(v + off)) & 3) == 0;
     for (int b = wave; b * kBlock < len; b += kWaves) {
@@ -172,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
         const float s = units_of(x & 127u) * um;
         M[i] = x & 128u ? -s : s;
         V[i] = units_of(y) * uv;
-        update(P[i], G[i], M[i], V[i], k, bc.x, bc.y);
+        update(P[i], G[i], M[i], V[i], k, bc.size, bc.inv_bc2_sqrt);
         if (i < n) {
           tm = max(tm, __float_as_uint(M[i]) & 0x7fffffffu);
           tv = max(tv, __float_as_uint(V[i]) & 0x7fffffffu);
@@ -281,7 +291,7 @@ extern "C" {
 
 int gps_adamw8_block(void) { return kBlock; }
 
-size_t gps_adamw8_workspace_floats(int64_t n_chunks) { return n_chunks > 0 ? (size_t)norm_blocks(n_chunks) + 1 + 2 * (size_t)n_chunks : 0; }
+size_t gps_adamw8_workspace_floats(int64_t n_chunks) { return n_chunks > 0 ? (size_t)norm_blocks(n_chunks) + 3 * (size_t)n_chunks : 0; }
 
 int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, const int64_t* chunk_off,
                     const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active, int64_t n_chunks, double* hyper,
@@ -290,11 +300,10 @@ int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m
   if (n_chunks == 0) return GPS_OK;
   GPS_REQUIRE(p && g && m && v && m_exp && v_exp && chunk_off && chunk_len && chunk_param && active && hyper && pstep && ws,
               "gps_adamw8_step: null pointer argument");
-  GPS_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 7) == 0, "gps_adamw8_step: workspace must be 8-byte aligned");
   GPS_REQUIRE(gps_optim_chunk() == kChunk, "gps_adamw8_step: chunk table of %d elements", gps_optim_chunk());
   hipStream_t s = gps::as_stream(stream);
   const int nb = norm_blocks(n_chunks);
-  float2* coef = reinterpret_cast<float2*>(ws + ((nb + 1) & ~1));   // per parameter: never more of them than chunks
+  ChunkCoef* coef = reinterpret_cast<ChunkCoef*>(ws + nb);
   k_sqnorm8<<<nb, kThreads, 0, s>>>(g, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, ws, coef);
   k_adamw8<<<(unsigned)(n_chunks < kStepBlocks ? n_chunks : kStepBlocks), kThreads, 0, s>>>(
       p, g, m, v, m_exp, v_exp, chunk_off, chunk_len, chunk_param, active, n_chunks, hyper, pstep, seed, ws, nb, coef);

@@ -257,3 +257,28 @@ def test_parameters_that_move_and_captured_steps():
     for x, y in zip(params, twin):
         # the arena offsets differ now, so the codes do; the update itself uses the unrounded moments
         assert (x - y).abs().max() <= 2.0 ** -22 * float(x.abs().max())
+
+
+def test_parameters_without_elements():
+    """More parameters than chunks: the empty ones have no chunk, and nothing of theirs is touched."""
+    from graphgps_amd.optim import FlatAdamW8bit
+    g = torch.Generator().manual_seed(3)
+    start, grads = torch.randn(700, generator=g), torch.randn(3, 700, generator=g)
+    out = []
+    for empties in (0, 5000):
+        params = [torch.nn.Parameter(torch.zeros(0, 4, device="cuda")) for _ in range(empties)] + [torch.nn.Parameter(start.cuda())]
+        opt = FlatAdamW8bit(params, lr=1e-2, max_grad_norm=1.0)
+        for gr in grads:
+            for p in params:
+                p.grad = torch.zeros_like(p)
+            params[-1].grad = gr.cuda()
+            opt.step()
+        state = opt.state_dict()["state"]
+        assert list(state) == [empties] and float(state[empties]["step"]) == 3
+        out.append((params[-1].detach(), state[empties]))
+        again = FlatAdamW8bit(params)
+        again.load_state_dict(opt.state_dict())
+        for a, b in zip(again.moments(), opt.moments()):
+            assert torch.equal(a, b)
+    (p0, s0), (p1, s1) = out
+    assert torch.equal(p0, p1) and all(torch.equal(s0[k], s1[k]) for k in ("exp_avg_sq_exp", "exp_avg_exp"))
