@@ -4,9 +4,17 @@
 // BN rows of K (both maps side by side) and V staged in LDS.  Scores are formed as S^T = K Q^T, so that a query is a lane's
 // column: the running maximum and sum of each map need two cross-lane steps per block, the rescaling of the accumulators is by
 // a per-lane scalar, and the weights feed O^T += V^T P^T from the registers they are in.  The two maps keep statistics and
-// accumulators of their own and meet once, in the epilogue.  Two blocks of K and V are in LDS: one is read while the next one
-// arrives, straight from memory, behind a single barrier per block.  Two wavefronts per SIMD let one's exponentials run under the
-// other's matrix instructions.
+// accumulators of their own (the first one's are those of the maps' difference, see `mix`) and meet once, in the epilogue.  Two blocks of
+// K and V are in LDS: one is read while the next one arrives, straight from memory, behind a single barrier per block.
+//
+// Bound by what a SIMD issues: at 64 columns a block of 16 x 32 pairs is 24 matrix instructions (16 cycles each) and about 150 vector
+// instructions, two exponentials per pair among them; three wavefronts per SIMD cover each other's waits for the barrier and for LDS
+// in part.  Two graphs of 4,175 and 5,261 nodes, 8 heads over 4 of 64 columns, bf16: 386 us = 720 TFLOP/s of the products that the
+// kernel makes (12 d flops per pair and head: both maps' weighted sums).  Matrix units busy 37 % of the time, vector units about half.
+// Four causal sequences of ~2,600 rows, 6 heads over 2 of 128 columns, fp16, dropped keys: 356-380 us.  256 molecules of ~31 nodes,
+// 8 heads of 24 columns, fp32: 42 us.
+// Tried and slower there: 8 wavefronts per workgroup (506 us: half the staging, but one workgroup per CU), 2 (752); other LDS
+// permutations with fewer bank conflicts on paper (394).
 #include <initializer_list>
 
 #include "diff_attn.hpp"
@@ -14,7 +22,9 @@
 namespace {
 using namespace diffattn;
 
-// keys per block: 64 where the registers hold two wavefronts per SIMD with it, else 32
+// Keys per block: 64 where the registers hold three wavefronts per SIMD with it, else 32.  16 bits, 32 columns (syntax trees of ~125 nodes):
+// 14.9 us with 64, 17.3 with 32; 64 columns (two graphs of ~4,700 nodes): 463 with 64, 386 with 32; fp32, 32 columns (molecules): 66 with
+// 64, 42 with 32.
 template <typename T, int DQ>
 constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
@@ -239,9 +249,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
   }
 }
 
+// QT = 1 everywhere: two tiles per wavefront halve its LDS reads but take the third wavefront's registers (two graphs of ~4,700
+// nodes, 64 columns: 440 us against 386; molecules in fp32: 72 against 42).
 template <typename T, int DQ, int QT>
 void launch_fwd(const Args& a, hipStream_t s) {
   const int per_wave = 16 * QT;
+  // Short segments: a workgroup as tall as the longest, no idle wavefronts in its barriers.  fp32, 8 heads of 24 columns: 1,024 graphs of 15
+  // nodes 73 us with 1, 79 with 2, 90 with 4; 512 of 30 nodes 49 with 2, 53 with 4 (the backward: 179, 185, 237 and 118, 140).
   const int waves = a.max_q > 0 && a.max_q <= per_wave ? 1 : a.max_q > 0 && a.max_q <= 2 * per_wave ? 2 : 4;
   const int tiles = (int)(a.Nq / (waves * per_wave)) + a.B + 1;
   const unsigned grid = (unsigned)xcd_grid(tiles * a.H);

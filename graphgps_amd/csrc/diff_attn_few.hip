@@ -3,8 +3,9 @@
 //
 // One WAVEFRONT per (unit of `cw` keys, key head): its 16 matrix columns are (query of the segment, head of the group) pairs, so
 // the heads that share keys read them once.  K goes straight from memory into fragments; V passes through 32 rows of LDS that
-// belong to the wavefront alone (no barrier anywhere) to be read down its columns.  HBM-bound: K and V are read once, 8 wavefronts
-// of a CU keep 8 x 16 KB of them in flight.  Units are tiles of k_ptr: a long segment has more of them, none waits for another.
+// belong to the wavefront alone (no barrier anywhere) to be read down its columns.  Units are tiles of k_ptr: a long segment has more of
+// them, none waits for another.  HBM-bound: K and V are read once.  One query over eight sequences of 33,000 keys, 8 heads over 2 of 64 columns, bf16:
+// 268 MB in 57 us = 4.7 TB/s (a large copy: 4.88) and 9 us for the join; walking whole sequences in one workgroup took 17 ms.
 #include "diff_attn.hpp"
 
 namespace diffattn {
@@ -271,19 +272,30 @@ __global__ __launch_bounds__(Waves * 64) void k_diff_join(Args a, int cw, int ca
 
 }  // namespace
 
-// Keys per unit: about 2,048 units (8 wavefronts on each of 256 CUs) where the keys suffice
+// Keys per unit: about 1,024 units (4 wavefronts on each of 256 CUs) where the keys suffice.  One query over eight sequences of 33,000
+// keys on average, 2 key heads of 64 columns, bf16, split + join: 512 units 92 + 7 us, 1,024 57 + 9, 2,048 62 + 14, 4,096 53 + 23.
 int few_unit_keys(const Args& a) {
   int cw = 64;
-  while (cw < 1024 && a.Nk * a.Hk > (int64_t)2048 * cw) cw *= 2;
+  while (cw < 1024 && a.Nk * a.Hk > (int64_t)1024 * cw) cw *= 2;
   return cw;
 }
 int64_t few_units(const Args& a) { return a.Nk / few_unit_keys(a) + a.B + 1; }
 int few_columns(const Args& a) { return a.max_q * (a.H / a.Hk); }
 
-// Few queries: all (query, head of a group) pairs of a segment fit two column blocks, the keys do not fit one unit, and the join's
-// grid of one workgroup per row stays far from the launch limit of 2^32 threads
+// Few queries: all (query, head of a group) pairs of a segment fit one column block, the keys do not fit one unit, and the join's grid
+// of one workgroup per row stays far from the launch limit of 2^32 threads.  Two column blocks, each of which walks the unit's keys,
+// where the form of diff_attn.hip would leave CUs idle, and in fp32, whose products are what takes the time.  Measured here / there (us;
+// 64 columns, 4 heads of their own or 8 that share keys; forward):
+//   columns  queries x keys x segments      bf16          fp32
+//         1   1 x 65 x 2,000              75 / 87      229 / 530
+//         1   1 x 400 x 300               47 / 47      252 / 279
+//        32   4 x 4,000 x 8               26 / 100      43 / 489
+//        32   32 x 4,000 x 8              58 / 99       96 / 488
+//        32   4 x 1,000 x 64              58 / 48       96 / 259
+//        32   32 x 4,000 x 64            264 / 199     873 / 973
 bool few_applies(const Args& a) {
-  return a.max_q > 0 && a.max_q <= 32 && few_columns(a) <= 32 && (a.max_k == 0 || a.max_k > 64) && a.Nk > 0 && a.Nq <= (1 << 20);
+  const int columns = a.dtype == GPS_F32 || (int64_t)a.B * a.H < 256 ? 32 : 16;
+  return a.max_q > 0 && a.max_q <= 32 && few_columns(a) <= columns && (a.max_k == 0 || a.max_k > 64) && a.Nk > 0 && a.Nq <= (1 << 20);
 }
 size_t few_workspace_floats(const Args& a) { return (size_t)few_units(a) * a.Hk * few_columns(a) * (4 * (size_t)a.d + 4); }
 
@@ -299,7 +311,9 @@ void forward_few(const Args& a, hipStream_t s) {
     k_diff_few<T, 128><<<grid, kUnitWaves * 64, 0, s>>>(a, cw, cap);
   const size_t lds = (4 * a.d + 4) * sizeof(float);
   const dim3 rows((unsigned)a.Nq, (unsigned)a.H);
-  if (few_units(a) > (int64_t)16 * (a.B + 1))   // long lists of units: 16 wavefronts walk one
+  // Long lists of units: 16 wavefronts walk one (33,000 keys on average, 2,048 units: 14 us against 35 with 4).  Short ones: 4 (32 queries
+  // of ~125 keys: 4.1 us against 4.6).
+  if (few_units(a) > (int64_t)16 * (a.B + 1))
     k_diff_join<T, 16><<<rows, 1024, 16 * lds, s>>>(a, cw, cap);
   else
     k_diff_join<T, 4><<<rows, 256, 4 * lds, s>>>(a, cw, cap);

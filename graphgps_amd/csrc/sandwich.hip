@@ -10,6 +10,10 @@
 // so that every element is read once; statistics are two-pass there (mean, then centred squares) in fp32, kept for the backward
 // as four floats per row, and y is recomputed from x and a in fp32 rather than re-read rounded.  The column sums stay in
 // registers while a workgroup walks its rows, leave once per workgroup, and a second launch adds them in a fixed order.
+//
+// 50,001 x 2,048, bf16, full gate: forward 191 us = 5.4 TB/s (a large copy: 4.88, half of it writes; here two streams in five),
+// backward 386 us = 4.2 TB/s (the four sums' and the fetched row's registers leave two workgroups per CU), column sums 5 us.
+// 7,681 x 384, fp32: 12.5, 23.5 and 4 us; a pass of both takes 160 us of host time.
 #include "gps_common.hpp"
 
 namespace {
@@ -426,7 +430,9 @@ void launch(const Args& a, bool backward, hipStream_t s) {
                                                                a.dpre_bias, a.dgate);
 }
 
-// lanes of a row and chunks of V elements per lane, by the number of chunks
+// Lanes of a row and chunks of V elements per lane, by the number of chunks.  Rows inside one wavefront need no barrier: 384 columns fp32 as
+// 64 lanes x 2 chunks 12.4 us forward, 23.8 backward, as 256 lanes x 1 22.1 and 28.9; 64 columns as 16 lanes 4.3 us, as 64 lanes 4.6.
+// Wider ones spread: 2,048 columns bf16 as 256 lanes x 1 chunk 191 and 386 us, as 64 x 4 191 and 500 (registers).
 template <typename T, int V>
 void by_width(const Args& a, bool backward, hipStream_t s) {
   const int chunks = (a.D + V - 1) / V;
