@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
     for (int c = 0; c < DVT; ++c) {
       const int x = c * 16 + g * 4;
       if (x >= dv) continue;
-      store4(static_cast<T*>(a.o) + at + x, acc[0][i][c] * inv[0] + acc[1][i][c] * with);
+      store_out4<T>(a, at + x, acc[0][i][c] * inv[0] + acc[1][i][c] * with);
       if (a.o2) store4(a.o2 + at + x, acc[1][i][c] * inv[1]);
     }
     if (a.lse && g == 0) {
@@ -301,12 +301,13 @@ int check(const char* who, const Args* a) {
   GPS_REQUIRE(a->q_ptr && a->k_ptr && a->lam, "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nq == 0 || (a->q && a->o), "%s: null pointer argument", who);
   GPS_REQUIRE(a->Nk == 0 || (a->k && a->v), "%s: null pointer argument", who);
-  GPS_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->o2) && aligned16(a->ws), "%s: pointers must be 16-byte aligned", who);
+  GPS_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->o) && aligned16(a->o2) && aligned16(a->o_rest) && aligned16(a->ws), "%s: pointers must be 16-byte aligned", who);
   GPS_REQUIRE(by8({a->q_rs, a->q_hs, a->q_ms, a->k_rs, a->k_hs, a->k_ms, a->v_rs, a->v_hs}), "%s: strides must be multiples of 8 elements", who);
   // the lanes' offsets within a block of rows are 32-bit
   for (int64_t x : {a->q_rs, a->k_rs, a->v_rs, a->do_rs}) GPS_REQUIRE(x >= 0 && x <= (1 << 22), "%s: row stride %lld", who, (long long)x);
   for (int64_t x : {a->q_ms, a->k_ms}) GPS_REQUIRE(x >= 0 && x <= (1 << 28), "%s: map stride %lld", who, (long long)x);
   GPS_REQUIRE((a->o2 == nullptr) == (a->lse == nullptr), "%s: o2 and lse come together", who);
+  GPS_REQUIRE(!a->o_rest || a->dtype != GPS_F32, "%s: o_rest is for 16-bit types", who);
   return GPS_OK;
 }
 

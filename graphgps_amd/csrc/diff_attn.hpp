@@ -89,6 +89,12 @@ __device__ __forceinline__ Frag<T> frag_pack(f32x4 a, f32x4 b) {
   }
   return f;
 }
+// what frag_pack lost, as a fragment of its own (16-bit types)
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_lost(f32x4 a, f32x4 b, const Frag<T>& f) {
+  const vec_t<T, 4> x = __builtin_shufflevector(f.v, f.v, 0, 1, 2, 3), y = __builtin_shufflevector(f.v, f.v, 4, 5, 6, 7);
+  return frag_pack<T>(a - __builtin_convertvector(x, f32x4), b - __builtin_convertvector(y, f32x4));
+}
 // A fragment of the TRANSPOSE of the row-major LDS tile `m` (row stride `ld`): row of A = column col0 + (l & 15), slots = rows
 // row0 .. row0 + 31 in frag_pack's order
 template <typename T>
@@ -131,6 +137,15 @@ __device__ __forceinline__ void store4(T* p, f32x4 x) {
     *reinterpret_cast<f32x4*>(p) = x;
   else
     *reinterpret_cast<vec_t<T, 4>*>(p) = __builtin_convertvector(x, vec_t<T, 4>);
+}
+
+// the output's four elements from `at` on, and what they lose by rounding: dO . o over a row of o enters every dS of that row, so an
+// o that is rounded there would leave its error in all of them (rows that see a few keys: as large as what is left of dS)
+template <typename T>
+__device__ __forceinline__ void store_out4(const Args& a, int64_t at, f32x4 x) {
+  store4(static_cast<T*>(a.o) + at, x);
+  if constexpr (sizeof(T) == 2)
+    if (a.o_rest) store4(static_cast<T*>(a.o_rest) + at, x - __builtin_convertvector(__builtin_convertvector(x, vec_t<T, 4>), f32x4));
 }
 
 __device__ __forceinline__ float load_lam(const Args& a, int h, const bf16*) {

@@ -17,10 +17,17 @@
 namespace diffattn {
 namespace {
 
+// dS in two 16-bit terms.  With one, the error of dQ and dK is 1.41 to 1.5 times that of a gradient that is rounded once at its end, and
+// more (up to 1.9) where heads are narrow and rows see few keys: the terms of a sum cancel and their errors do not.  Up to 32
+// columns, where both second products of dS are small, it is kept in two: 1.1 to 1.3 times, for 20.6 us instead of 18.5 on 32 trees of ~123
+// nodes and 503 instead of 456 for a whole pass over 9 causal graphs of 2,108 (4 heads over 1, 16 columns).  Above that in one.
+template <typename T, int DQ>
+constexpr bool two_terms() { return sizeof(T) == 2 && DQ == 32; }
+
 constexpr int kDeltaRows = 64;   // rows of one k_diff_delta workgroup
 
 // D2 = dO . O2 and D1 = dO . O + lam D2: sixteen lanes per (row, head), sixteen rows of a head at a time.  HBM-bound: 9,436 rows of 8 heads
-// of 128 columns, bf16 with fp32 O2: 77 MB in 13 us.
+// of 128 columns, bf16 with what O lost and fp32 O2: 97 MB in 16 us.
 template <typename T>
 __global__ __launch_bounds__(256) void k_diff_delta(Args a, float* __restrict__ delta) {
   const int h = blockIdx.y, lane = threadIdx.x & 15, dv = 2 * a.d;
@@ -32,13 +39,16 @@ __global__ __launch_bounds__(256) void k_diff_delta(Args a, float* __restrict__ 
     if (r < a.Nq && a.lse[(int64_t)h * a.Nq + r] < kInf) {   // a row that saw no key has no gradient, whatever dO holds there
       const T* dop = static_cast<const T*>(a.dout) + r * a.do_rs + h * a.do_hs;
       const T* op = static_cast<const T*>(a.o) + (r * a.H + h) * dv;
+      const T* restp = static_cast<const T*>(a.o_rest) + (r * a.H + h) * dv;
       const float* o2p = a.o2 + (r * a.H + h) * dv;
       for (int c = lane * 4; c < dv; c += 64) {
         const vec_t<T, 4> go = *reinterpret_cast<const vec_t<T, 4>*>(dop + c), o = *reinterpret_cast<const vec_t<T, 4>*>(op + c);
         const f32x4 o2 = *reinterpret_cast<const f32x4*>(o2p + c);
+        vec_t<T, 4> rest = vec_t<T, 4>(0);
+        if (sizeof(T) == 2 && a.o_rest) rest = *reinterpret_cast<const vec_t<T, 4>*>(restp + c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x += (float)go[i] * (float)o[i];
+          x += (float)go[i] * ((float)o[i] + (float)rest[i]);
           y += (float)go[i] * o2[i];
         }
       }
@@ -213,12 +223,16 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
         }
       }
     }
-    Frag<T> w[KT], ds[2][KT];
+    Frag<T> w[KT], ds[2][KT], lost[2][KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       w[i] = frag_pack<T>(dp[i][0], dp[i][1]);
       ds[0][i] = frag_pack<T>(s[0][i][0], s[0][i][1]);
       ds[1][i] = frag_pack<T>(s[1][i][0], s[1][i][1]);
+      if constexpr (two_terms<T, DQ>()) {
+        lost[0][i] = frag_lost<T>(s[0][i][0], s[0][i][1], ds[0][i]);
+        lost[1][i] = frag_lost<T>(s[1][i][0], s[1][i][1], ds[1][i]);
+      }
     }
 #pragma unroll
     for (int c = 0; c < DVT; ++c) {
@@ -232,7 +246,10 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
       for (int c = 0; c < DQT; ++c) {
         const Frag<T> qf = L::frag_tr(lq, 0, m * DQ + c * 16, lane);
 #pragma unroll
-        for (int i = 0; i < KT; ++i) gk[m][i][c] = mma(qf, ds[m][i], gk[m][i][c]);
+        for (int i = 0; i < KT; ++i) {
+          gk[m][i][c] = mma(qf, ds[m][i], gk[m][i][c]);
+          if constexpr (two_terms<T, DQ>()) gk[m][i][c] = mma(qf, lost[m][i], gk[m][i][c]);
+        }
       }
    }
   }
@@ -390,14 +407,20 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      Frag<T> ds[QT];
+      Frag<T> ds[QT], lost[QT];
 #pragma unroll
-      for (int i = 0; i < QT; ++i) ds[i] = frag_pack<T>(s[m][i][0], s[m][i][1]);
+      for (int i = 0; i < QT; ++i) {
+        ds[i] = frag_pack<T>(s[m][i][0], s[m][i][1]);
+        if constexpr (two_terms<T, DQ>()) lost[i] = frag_lost<T>(s[m][i][0], s[m][i][1], ds[i]);
+      }
 #pragma unroll
       for (int c = 0; c < DQT; ++c) {
         const Frag<T> kf = L::frag_tr(lk, 0, m * DQ + c * 16, lane);
 #pragma unroll
-        for (int i = 0; i < QT; ++i) gq[m][i][c] = mma(kf, ds[i], gq[m][i][c]);
+        for (int i = 0; i < QT; ++i) {
+          gq[m][i][c] = mma(kf, ds[i], gq[m][i][c]);
+          if constexpr (two_terms<T, DQ>()) gq[m][i][c] = mma(kf, lost[i], gq[m][i][c]);
+        }
       }
     }
   }

@@ -264,7 +264,10 @@ __global__ __launch_bounds__(Waves * 64) void k_diff_join(Args a, int cw, int ca
 #pragma unroll
       for (int j = 0; j < Waves; ++j) o[i] += w[i][j] * lds[j * 2 * dv + i * dv + x];
     const int64_t at = (row * a.H + h) * dv + x;
-    static_cast<T*>(a.o)[at] = (T)(o[0] - lam * o[1]);
+    const float out = o[0] - lam * o[1];
+    static_cast<T*>(a.o)[at] = (T)out;
+    if constexpr (sizeof(T) == 2)
+      if (a.o_rest) static_cast<T*>(a.o_rest)[at] = (T)(out - (float)(T)out);
     if (a.o2) a.o2[at] = o[1];
   }
   if (a.lse && threadIdx.x < 2) a.lse[((int64_t)threadIdx.x * a.H + h) * a.Nq + row] = threadIdx.x ? lse[1] : lse[0];

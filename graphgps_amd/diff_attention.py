@@ -100,15 +100,21 @@ class _Call:
         a.k_rs, a.k_hs, a.k_ms = k.stride()[:3]
         a.v_rs, a.v_hs = v.stride()[:2]
         if kept is not None and n:
-            at = kept.data_ptr()
-            a.o2, a.lse = at, at + 4 * n * self.H * 2 * self.d
+            at, size = kept.data_ptr(), n * self.H * 2 * self.d
+            a.o2, a.lse = at, at + 4 * size
+            if q.dtype != torch.float32:                     # behind both, on 16 bytes
+                a.o_rest = at + (4 * (size + 2 * n * self.H) + 15) // 16 * 16
         return a
 
     def forward(self, q, k, v, lam, train: bool):
-        """-> (o, kept): ``kept`` is one fp32 buffer, the second map's share [Nq, H, 2d] and then the log-sums [2, H, Nq]."""
+        """-> (o, kept): ``kept`` is one fp32 buffer, the second map's share [Nq, H, 2d], then the log-sums [2, H, Nq], and for 16-bit
+        types what ``o`` lost when it was rounded [Nq, H, 2d]."""
         dev, n, L = q.device, q.shape[0], _lib.load()
         o = torch.empty(n, self.H, 2 * self.d, dtype=q.dtype, device=dev)
-        kept = torch.empty(n * self.H * (2 * self.d + 2), dtype=torch.float32, device=dev) if train else None
+        kept = None
+        if train:
+            rest = 0 if q.dtype == torch.float32 else n * self.H * self.d + 3
+            kept = torch.empty(n * self.H * (2 * self.d + 2) + rest, dtype=torch.float32, device=dev)
         self.args = a = self.block(q, k, v, lam, o, kept)
         a.ws_floats = L.gps_diff_attn_fwd_workspace_floats(ctypes.addressof(a))
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev) if a.ws_floats else None

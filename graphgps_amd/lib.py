@@ -203,7 +203,7 @@ class DiffAttn(ctypes.Structure):
                 + [(n, c_int64) for n in ("q_rs", "q_hs", "q_ms", "k_rs", "k_hs", "k_ms", "v_rs", "v_hs")]
                 + [(n, c_void_p) for n in ("q_ptr", "k_ptr", "keep")] + [("Nq", c_int64), ("Nk", c_int64)]
                 + [(n, c_int32) for n in ("B", "H", "Hk", "d", "causal", "lam_f32", "dtype", "max_q", "max_k")]
-                + [("scale", c_float)] + [(n, c_void_p) for n in ("o", "o2", "lse", "dout")]
+                + [("scale", c_float)] + [(n, c_void_p) for n in ("o", "o2", "lse", "o_rest", "dout")]
                 + [("do_rs", c_int64), ("do_hs", c_int64)] + [(n, c_void_p) for n in ("dq", "dk", "dv", "dlam")]
                 + [(n, c_int64) for n in ("dq_rs", "dq_hs", "dq_ms", "dk_rs", "dk_hs", "dk_ms", "dv_rs", "dv_hs")]
                 + [("ws", c_void_p), ("ws_floats", c_size_t)])

@@ -740,7 +740,8 @@ int gps_adamw_step(float* p, const float* g, float* m, float* v, const int64_t* 
  * strides multiples of 8 elements, row
  * strides up to 2^22 and map strides up to 2^28.  max_q / max_k: the longest segment if the host knows it, else 0; they choose
  * the launch shape only.
- * Training keeps o2 [Nq, H, 2d] (fp32, the second map's share of o) and lse [2, H, Nq] (fp32); both NULL at inference.
+ * Training keeps o2 [Nq, H, 2d] (fp32, the second map's share of o) and lse [2, H, Nq] (fp32); both NULL at inference.  For 16-bit
+ * types o_rest [Nq, H, 2d] (of that type), where given, takes what o lost when it was rounded, for the backward's row sums.
  * ws: gps_diff_attn_fwd_workspace_floats() floats of the same argument block (0 unless max_q says that there are few queries: then
  * the keys are split and joined), gps_diff_attn_bwd_workspace_floats() in the backward; 16-byte aligned.  The results do not depend on how work is split: no atomics. */
 #define GPS_F32 0
@@ -757,6 +758,7 @@ typedef struct gps_diff_attn {
   void* o; /* [Nq, H, 2d] contiguous */
   float* o2;
   float* lse;
+  void* o_rest;
   /* backward only */
   const void* dout;
   int64_t do_rs, do_hs;

@@ -380,3 +380,22 @@ def test_packed_projection_that_comes_back_elsewhere(how):
     got = torch.autograd.grad(o, [qkv, lam], do)
     del junk
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("max_q", [0, 1])
+def test_a_row_with_one_key_has_no_gradient_of_its_scores(dtype, max_q):
+    """One key: both maps' weights are 1 whatever the scores, so dS = dP - dO . O1 = 0.  What may be left of it: the weight that the
+    values meet is 1 - lam in 16 bits, half a step off and the same for all columns; what O lost, to 16 bits; the sums' fp32.  (An O
+    that is rounded in that difference would leave half a step of every column.)"""
+    n, H, d = 200, 4, 32
+    q, k, v, lam, qp, kp, do = make([1] * n, [1] * n, H, H, d, dtype, seed=9)
+    _, dq, dk, _, _ = run(q, k, v, lam, qp, kp, do, max_q=max_q, max_k=100 * max_q)
+    v, do, l = v.double().cpu(), do.double().cpu(), lam.double().cpu()[None]
+    half, size, dot = HALF[dtype], (v * do).abs().sum(-1), (v * do).sum(-1).abs()
+    lost = half * (1 - l) * dot + half ** 2 * 1.01 * (1 - l) * size + (2.0 ** -25 * do.abs().sum(-1) if dtype == F16 else 0.0)
+    ds = (lost + 2.0 ** -24 * (2 * d + 16) * (2 + l) * size) * (1 + 2 * half)
+    for got, other in ((dq, k), (dk, q)):
+        got, other = got.double().cpu().abs(), other.double().cpu().abs()
+        bound = ds[:, :, None, None] * d ** -0.5 * other * (1 + 2 * half) + 2.0 ** -25
+        assert (got <= bound).all(), float((got / bound).max())
