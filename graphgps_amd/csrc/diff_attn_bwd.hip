@@ -7,8 +7,8 @@
 // queries and workgroups that own queries and walk the keys (the scores and dP twice, but no atomics: every sum in one fixed order).
 //
 // Two graphs of 4,175 and 5,261 nodes, 8 heads over 4 of 64 columns, bf16: 1.17 ms = 550 TFLOP/s of its 28 d flops per pair and head (20 d
-// with the scores and dP once).  No unit is saturated: LDS 45 % busy (every fragment that a wavefront reads there serves one 16 x 16
-// tile), vector units 39 %, matrix units 26 %; 213 registers leave two wavefronts per SIMD, which wait for each other's phases.
+// with the scores and dP once).  No unit is saturated: LDS 42 % busy (every fragment that a wavefront reads there serves one 16 x 16
+// tile), vector units 40 %, matrix units 27 %; 213 registers leave two wavefronts per SIMD, which wait for each other's phases.
 // Tried and slower: two tiles per wavefront (373 registers, one wavefront per SIMD: 1.51 ms; for dQ alone, spilling: 1.44), three
 // wavefronts per SIMD (28 registers spilled: 1.29), eight wavefronts per workgroup (half the staging: 1.18-1.22), a copy of the step
 // without the mask's selects (1.16, and 90 against 86 us in fp32).
