@@ -4,17 +4,21 @@
 // BN rows of K (both maps side by side) and V staged in LDS.  Scores are formed as S^T = K Q^T, so that a query is a lane's
 // column: the running maximum and sum of each map need two cross-lane steps per block, the rescaling of the accumulators is by
 // a per-lane scalar, and the weights feed O^T += V^T P^T from the registers they are in.  The two maps keep statistics and
-// accumulators of their own (the first one's are those of the maps' difference, see `mix`) and meet once, in the epilogue.  Two blocks of
-// K and V are in LDS: one is read while the next one arrives, straight from memory, behind a single barrier per block.
+// accumulators of their own and meet once, in the epilogue.  Two blocks of K and V are in LDS: one is read while the next one arrives,
+// straight from memory, behind a single barrier per block.
 //
-// Bound by what a SIMD issues: at 64 columns a block of 16 x 32 pairs is 24 matrix instructions (16 cycles each) and about 150 vector
-// instructions, two exponentials per pair among them; three wavefronts per SIMD cover each other's waits for the barrier and for LDS
-// in part.  Two graphs of 4,175 and 5,261 nodes, 8 heads over 4 of 64 columns, bf16: 386 us = 720 TFLOP/s of the products that the
-// kernel makes (12 d flops per pair and head: both maps' weighted sums).  Matrix units busy 37 % of the time, vector units about half.
-// Four causal sequences of ~2,600 rows, 6 heads over 2 of 128 columns, fp16, dropped keys: 356-380 us.  256 molecules of ~31 nodes,
-// 8 heads of 24 columns, fp32: 42 us.
-// Tried and slower there: 8 wavefronts per workgroup (506 us: half the staging, but one workgroup per CU), 2 (752); other LDS
-// permutations with fewer bank conflicts on paper (394).
+// In 16 bits a weight enters the second product in two terms, its rounding and what that lost (frag_lost).  The maps nearly cancel where
+// they agree, and a single rounding of each leaves its error on that small difference: relative to the value rounded once at the end, the
+// error of o is 1.0 times with two terms and 1.4 to 1.55 times with one on independent maps (0.0017 against 0.0025; two graphs of ~4,700
+// nodes 497 against 353 us, trees 14.5 against 11.7, ordered sequences 401 against 373), and 1 / (1 - lam) times and more where they
+// resemble each other.  Rounding the difference of the maps' weights instead needs the ratio of their final sums while it is formed: a
+// ratio from the keys seen so far puts errors into the sum that go by a key's weight when it was met, not by its weight at the end.
+//
+// Bound by the matrix units and what a SIMD issues around them: at 64 columns a block of 16 x 32 pairs is 40 matrix instructions (16
+// cycles each) and about 190 vector instructions, two exponentials per pair among them.  Two graphs of 4,175 and 5,261 nodes, 8 heads over
+// 4 of 64 columns, bf16: 497 us = 930 TFLOP/s of the products that the kernel makes (20 d flops per pair and head; 8 d are the
+// operator's), where a large matrix product reaches 1,262.  Four causal sequences of ~2,600 rows, 6 heads over 2 of 128 columns, fp16,
+// dropped keys: 401 us.  256 molecules of ~31 nodes, 8 heads of 24 columns, fp32: 42 us; 32 trees of ~123 nodes, 4 heads of 32, bf16: 14.5.
 #include <initializer_list>
 
 #include "diff_attn.hpp"
@@ -23,8 +27,8 @@ namespace {
 using namespace diffattn;
 
 // Keys per block: 64 where the registers hold three wavefronts per SIMD with it, else 32.  16 bits, 32 columns (syntax trees of ~125 nodes):
-// 14.9 us with 64, 17.3 with 32; 64 columns (two graphs of ~4,700 nodes): 463 with 64, 386 with 32; fp32, 32 columns (molecules): 66 with
-// 64, 42 with 32.
+// 14.5 us with 64, 14.9 with 32, and 16.9 against 19.6 with dropped keys; 64 columns (two graphs of ~4,700 nodes): 775 with 64, 497 with
+// 32; fp32, 32 columns (molecules): 66 with 64, 42 with 32.
 template <typename T, int DQ>
 constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
@@ -86,12 +90,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
       }
   }
   const int all_see = a.causal ? t.local + wave * QT * 16 + shift + 1 : nk;   // keys that every query of this wavefront sees
-  // acc[0] = sum (p1 - mix p2) v and acc[1] = sum p2 v with p_i = 2^(score - ref_i): see `mix` below
-  f32x4 acc[2][QT][DVT];
-  float ref[2][QT], sum[2][QT], mix[QT];
+  f32x4 acc[2][QT][DVT];   // of each map: sum p v with p = 2^(score - ref)
+  float ref[2][QT], sum[2][QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    mix[i] = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       ref[m][i] = -kLowest;
@@ -142,7 +144,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
           }
       }
     }
-    // The references move only when a score passes one by more than 2^6: weights stay below 64, far inside every type, and the
+    // The references move only when a score passes one by more than 6: weights stay below 2^6, far inside every type, and the
     // accumulators are rescaled a few times per row instead of at every new maximum.
     float hi[2][QT];   // over this lane's keys
     bool past = false;
@@ -183,32 +185,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
           }
         sum[m][i] += add;
       }
-    // The maps nearly cancel where they agree.  Rounding p1 and p2 to 16 bits apart would leave both errors on that small
-    // difference, so what is rounded is p1 - mix p2, with mix = lam times the ratio of the sums so far: at the end acc[1] enters
-    // with the little that the ratio has moved since.  Changing mix is exact in the accumulators:
-    // sum (p1 - mix' p2) v = acc[0] + (mix - mix') acc[1].
-    if (move) {
+    Frag<T> p[2][QT][BN / 32], lost[2][QT][BN / 32];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float l1 = over_groups(sum[0][i], [](float u, float v) { return u + v; });
-        const float l2 = over_groups(sum[1][i], [](float u, float v) { return u + v; });
-        const float to = l2 > 0.f ? lam * l1 * __builtin_amdgcn_rcpf(l2) : 0.f;
-        const float with = mix[i] * f[0][i] - to * f[1][i];
-        mix[i] = to;
+        if (move) {
 #pragma unroll
-        for (int c = 0; c < DVT; ++c) {
-          acc[0][i][c] = acc[0][i][c] * f[0][i] + acc[1][i][c] * with;
-          acc[1][i][c] *= f[1][i];
+          for (int c = 0; c < DVT; ++c) acc[m][i][c] *= f[m][i];
         }
-      }
-    }
-    Frag<T> p[2][QT][BN / 32];
 #pragma unroll
-    for (int i = 0; i < QT; ++i)
-#pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) {
-        p[0][i][kk] = frag_pack<T>(s[0][i][2 * kk] - s[1][i][2 * kk] * mix[i], s[0][i][2 * kk + 1] - s[1][i][2 * kk + 1] * mix[i]);
-        p[1][i][kk] = frag_pack<T>(s[1][i][2 * kk], s[1][i][2 * kk + 1]);
+        for (int kk = 0; kk < BN / 32; ++kk) {
+          p[m][i][kk] = frag_pack<T>(s[m][i][2 * kk], s[m][i][2 * kk + 1]);
+          if constexpr (sizeof(T) == 2) lost[m][i][kk] = frag_lost<T>(s[m][i][2 * kk], s[m][i][2 * kk + 1], p[m][i][kk]);
+        }
       }
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk)
@@ -219,6 +209,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
         for (int i = 0; i < QT; ++i) {
           acc[0][i][c] = mma(vf, p[0][i][kk], acc[0][i][c]);
           acc[1][i][c] = mma(vf, p[1][i][kk], acc[1][i][c]);
+          if constexpr (sizeof(T) == 2) {
+            acc[0][i][c] = mma(vf, lost[0][i][kk], acc[0][i][c]);
+            acc[1][i][c] = mma(vf, lost[1][i][kk], acc[1][i][c]);
+          }
         }
       }
   }
@@ -234,12 +228,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
     }
     if (row[i] < 0) continue;
     const int64_t at = (row[i] * a.H + h) * dv;
-    const float with = mix[i] * inv[0] - lam * inv[1];
 #pragma unroll
     for (int c = 0; c < DVT; ++c) {
       const int x = c * 16 + g * 4;
       if (x >= dv) continue;
-      store_out4<T>(a, at + x, acc[0][i][c] * inv[0] + acc[1][i][c] * with);
+      store_out4<T>(a, at + x, acc[0][i][c] * inv[0] - acc[1][i][c] * (lam * inv[1]));
       if (a.o2) store4(a.o2 + at + x, acc[1][i][c] * inv[1]);
     }
     if (a.lse && g == 0) {
@@ -250,7 +243,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
 }
 
 // QT = 1 everywhere: two tiles per wavefront halve its LDS reads but take the third wavefront's registers (two graphs of ~4,700
-// nodes, 64 columns: 440 us against 386; molecules in fp32: 72 against 42).
+// nodes, 64 columns: 786 us against 497; trees 17.0 against 14.5; molecules in fp32: 62 against 42).
 template <typename T, int DQ, int QT>
 void launch_fwd(const Args& a, hipStream_t s) {
   const int per_wave = 16 * QT;

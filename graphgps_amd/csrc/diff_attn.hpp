@@ -76,7 +76,8 @@ __device__ __forceinline__ Frag<T> frag_zero() {
   return f;
 }
 // two result tiles -> the B fragment over their 32 rows.  16-bit types round to nearest here: the weights and their
-// gradients enter the second product in the input's type, which is what the matrix instruction takes.
+// gradients enter the second product in the input's type, which is what the matrix instruction takes; frag_lost makes a second
+// operand of what that rounding lost.
 template <typename T>
 __device__ __forceinline__ Frag<T> frag_pack(f32x4 a, f32x4 b) {
   Frag<T> f;
