@@ -45,8 +45,7 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
           q[m][s] = frag_load(static_cast<const T*>(a.q) + (int64_t)(q0 + qi) * a.q_rs + h * a.q_hs + m * a.q_ms + s * 32 + g * 8);
       }
     f32x4 acc[2][DVT];
-    float top[2] = {-kInf, -kInf}, sum[2] = {0.f, 0.f}, mix = 0.f;
-    const float lam = have ? load_lam(a, h, static_cast<const T*>(nullptr)) : 0.f;
+    float top[2] = {-kInf, -kInf}, sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < DVT; ++x) acc[0][x] = acc[1][x] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -129,22 +128,26 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
           }
         sum[m] = sum[m] * f[m] + add;
       }
-      // as in diff_attn.hip: what is rounded is p1 - mix p2, near the difference that is wanted
-      const float l1 = over_groups(sum[0], [](float x, float y) { return x + y; });
-      const float l2 = over_groups(sum[1], [](float x, float y) { return x + y; });
-      const float to = l2 > 0.f ? lam * l1 * __builtin_amdgcn_rcpf(l2) : 0.f, with = mix * f[0] - to * f[1];
-      mix = to;
 #pragma unroll
-      for (int x = 0; x < DVT; ++x) {
-        acc[0][x] = acc[0][x] * f[0] + acc[1][x] * with;
-        acc[1][x] *= f[1];
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int x = 0; x < DVT; ++x) acc[m][x] *= f[m];
       }
-      const Frag<T> p0 = frag_pack<T>(s[0][0] - s[1][0] * mix, s[0][1] - s[1][1] * mix), p1 = frag_pack<T>(s[1][0], s[1][1]);
+      const Frag<T> p0 = frag_pack<T>(s[0][0], s[0][1]), p1 = frag_pack<T>(s[1][0], s[1][1]);
+      Frag<T> lost0, lost1;   // weights in two terms, as in diff_attn.hip
+      if constexpr (sizeof(T) == 2) {
+        lost0 = frag_lost<T>(s[0][0], s[0][1], p0);
+        lost1 = frag_lost<T>(s[1][0], s[1][1], p1);
+      }
 #pragma unroll
       for (int x = 0; x < DVT; ++x) {
         const Frag<T> vf = frag_tr(lv, LV, 0, x * 16, lane);
         acc[0][x] = mma(vf, p0, acc[0][x]);
         acc[1][x] = mma(vf, p1, acc[1][x]);
+        if constexpr (sizeof(T) == 2) {
+          acc[0][x] = mma(vf, lost0, acc[0][x]);
+          acc[1][x] = mma(vf, lost1, acc[1][x]);
+        }
       }
     }
     float* part = a.ws + (((int64_t)unit * a.Hk + hk) * cap + c) * part_floats(dv);
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
       if (!have) continue;
 #pragma unroll
       for (int x = 0; x < DVT; ++x)
-        if (x * 16 + g * 4 < dv) *reinterpret_cast<f32x4*>(part + m * dv + x * 16 + g * 4) = m ? acc[1][x] : acc[0][x] + acc[1][x] * mix;
+        if (x * 16 + g * 4 < dv) *reinterpret_cast<f32x4*>(part + m * dv + x * 16 + g * 4) = acc[m][x];
       if (g == 0) {
         part[2 * dv + 2 * m] = top[m];
         part[2 * dv + 2 * m + 1] = z;
@@ -290,12 +293,12 @@ int few_columns(const Args& a) { return a.max_q * (a.H / a.Hk); }
 // where the form of diff_attn.hip would leave CUs idle, and in fp32, whose products are what takes the time.  Measured here / there (us;
 // 64 columns, 4 heads of their own or 8 that share keys; forward):
 //   columns  queries x keys x segments      bf16          fp32
-//         1   1 x 65 x 2,000              75 / 87      229 / 530
-//         1   1 x 400 x 300               47 / 47      252 / 279
-//        32   4 x 4,000 x 8               26 / 100      43 / 489
-//        32   32 x 4,000 x 8              58 / 99       96 / 488
-//        32   4 x 1,000 x 64              58 / 48       96 / 259
-//        32   32 x 4,000 x 64            264 / 199     873 / 973
+//         1   1 x 65 x 2,000              75 / 100     225 / 527
+//         1   1 x 400 x 300               48 / 52      247 / 280
+//        32   4 x 4,000 x 8               26 / 144      42 / 488
+//        32   32 x 4,000 x 8              57 / 144      93 / 488
+//        32   4 x 1,000 x 64              71 / 64       95 / 259
+//        32   32 x 4,000 x 64            257 / 197     873 / 974
 bool few_applies(const Args& a) {
   const int columns = a.dtype == GPS_F32 || (int64_t)a.B * a.H < 256 ? 32 : 16;
   return a.max_q > 0 && a.max_q <= 32 && few_columns(a) <= columns && (a.max_k == 0 || a.max_k > 64) && a.Nk > 0 && a.Nq <= (1 << 20);

@@ -124,7 +124,7 @@ def test_large_values_that_end_with_little_weight(kind, max_q, dtype):
 
 @TYPES
 @pytest.mark.parametrize("n", [64, 900])
-@pytest.mark.parametrize("max_q", [0])
+@pytest.mark.parametrize("max_q", [0, 1])
 def test_map_that_hands_over(max_q, n, dtype):
     """The first map rests on key 0.  The second one starts among the keys behind it, whose values are large, and moves to later keys
     with all its weight: nothing of those values may be left."""
