@@ -32,6 +32,13 @@ using namespace diffattn;
 template <typename T, int DQ>
 constexpr int block_keys() { return sizeof(T) * DQ <= 64 ? 64 : 32; }
 
+// A row's largest weight is 2^kUp when its reference is set.  float16 weights below 2^-25 round to zero, and a long row may have a share
+// of its sum in keys that far below its largest, so the largest is put near the top of the type (2^(9 + 6) < 65504).
+template <typename T>
+constexpr float kUp = 0.f;
+template <>
+constexpr float kUp<f16> = 9.f;
+
 template <typename T, int DQ, int QT, bool Masked>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2) : DQ == 32 ? 3 : 1) void k_diff_fwd(Args a, int tile_count) {
   constexpr int DV = 2 * DQ, DVT = DV / 16, ST = DQ / 32, BN = block_keys<T, DQ>(), KT = BN / 16;
@@ -144,8 +151,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
           }
       }
     }
-    // The references move only when a score passes one by more than 6: weights stay below 2^6, far inside every type, and the
-    // accumulators are rescaled a few times per row instead of at every new maximum.
+    // The references move only when a score passes one by more than 6 + kUp: weights stay below 2^(6 + kUp), inside every type, and
+    // the accumulators are rescaled a few times per row instead of at every new maximum.
     float hi[2][QT];   // over this lane's keys
     bool past = false;
 #pragma unroll
@@ -156,7 +163,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
 #pragma unroll
         for (int j = 1; j + 1 < 4 * KT; j += 2) x = maximum(maximum(x, s[m][i][j / 4][j % 4]), s[m][i][(j + 1) / 4][(j + 1) % 4]);
         hi[m][i] = maximum(x, s[m][i][KT - 1][3]);
-        past |= __builtin_fmaf(hi[m][i], scale2, -ref[m][i]) > 6.f;
+        past |= __builtin_fmaf(hi[m][i], scale2, -ref[m][i]) > 6.f + kUp<T>;
       }
     const bool move = __any(past);
     float f[2][QT];
@@ -165,7 +172,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
-          const float now = fmaxf(ref[m][i], over_groups(hi[m][i], [](float u, float v) { return maximum(u, v); }) * scale2);
+          const float now = fmaxf(ref[m][i], over_groups(hi[m][i], [](float u, float v) { return maximum(u, v); }) * scale2 - kUp<T>);
           f[m][i] = __builtin_amdgcn_exp2f(ref[m][i] - now);
           ref[m][i] = now;
           sum[m][i] *= f[m][i];

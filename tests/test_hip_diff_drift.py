@@ -138,3 +138,27 @@ def test_map_that_hands_over(max_q, n, dtype):
     v[1:32] *= 300.0
     got = run(q, k, v, lam, qp, kp, do, scale=1.0, max_q=max_q)
     compare(got, (q, k, v, lam, qp, kp), do, dtype, scale=1.0)
+
+
+@TYPES
+@pytest.mark.parametrize("max_q", [0, 1])
+def test_long_row_with_a_share_far_below_its_peak(max_q, dtype):
+    """A peak of the first map and 2^20 keys at 2^-25.6 of it, 2 % of the row together: weights that float16 does not hold as they
+    are.  The bound counts fp32 sums as they are made: 16-bit products come 32 keys to an addition, fp32 products (whose weights
+    need no help: the type is there to see that they stay as they were) one by one, n additions of half a step of a sum that does not
+    exceed the mass.  float16 adds what may round to zero:
+    2^-25 of a peak at 2^9 for each key, and in the split form 2^-25 of the peak for the at most 1,024 keys of its unit."""
+    from graphgps_amd import ops
+    n = 1 << 20
+    g = torch.Generator().manual_seed(7)
+    q, k = torch.zeros(1, 1, 2, 8), torch.zeros(n, 1, 2, 8)
+    q[..., 0] = 1.0
+    k[1:, :, 0, 0] = -25.6 * LN2
+    v = torch.rand(n, 1, 16, generator=g) + 0.5
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    lam, qp, kp = torch.tensor([0.5]).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda()
+    with torch.no_grad():
+        got = ops.diff_attention(q, k, v, lam, qp, kp, scale=1.0, max_q=max_q)
+    want, mass, w, _ = reference(q, k, v, lam, qp, kp, scale=1.0)
+    lost = 0.0 if dtype != F16 else n * 2.0 ** -34 if max_q == 0 else 1024 * 2.0 ** -25
+    close(got, want["o"], mass["o"], w + 2 * HALF[dtype] + (n + 16 if dtype == F32 else n // 32 + 64) * 2.0 ** -24 + lost, "o")
