@@ -42,7 +42,12 @@ def _check_ptr(p: torch.Tensor, name: str, dev) -> torch.Tensor:
               f"{tuple(getattr(p, 'shape', ()))}")
     if p.device != dev:
         _fail(f"diff_attention: {name} is on {p.device}, q on {dev}")
-    return p.to(torch.int32).contiguous()
+    return _keepable(p.to(torch.int32).contiguous())
+
+
+def _keepable(t: torch.Tensor) -> torch.Tensor:
+    """autograd saves no tensor that was made under inference mode (a batch's index may have been): a copy then."""
+    return t.clone() if t.is_inference() and not torch.is_inference_mode_enabled() else t
 
 
 def _check_inputs(q, k, v, lam, key_mask) -> Tuple[int, int, int]:
@@ -88,12 +93,17 @@ class _Call:
         self.scale = float(d) ** -0.5 if scale is None else float(scale)
         self.max_q, self.max_k = int(max_q), int(max_k)
         self.q_ptr, self.k_ptr = q_ptr, k_ptr
-        self.keep = None if key_mask is None else key_mask.contiguous().view(torch.uint8)
+        self.keep = None if key_mask is None else _keepable(key_mask.contiguous().view(torch.uint8))
 
-    def block(self, q, k, v, lam, o, kept) -> DiffAttn:
+    def segments(self):
+        """What the kernels read beside the operands.  The backward reads it too, so it is saved like an operand: a change in place in
+        between raises there."""
+        return self.q_ptr, self.k_ptr, self.keep
+
+    def block(self, q, k, v, lam, o, kept, q_ptr, k_ptr, keep) -> DiffAttn:
         n = q.shape[0]
-        a = DiffAttn(q=ptr(q), k=ptr(k), v=ptr(v), lam=ptr(lam), o=ptr(o), q_ptr=ptr(self.q_ptr), k_ptr=ptr(self.k_ptr), keep=ptr(self.keep),
-                     Nq=n, Nk=k.shape[0], B=self.q_ptr.numel() - 1, H=self.H, Hk=self.Hk, d=self.d, causal=int(self.causal),
+        a = DiffAttn(q=ptr(q), k=ptr(k), v=ptr(v), lam=ptr(lam), o=ptr(o), q_ptr=ptr(q_ptr), k_ptr=ptr(k_ptr), keep=ptr(keep),
+                     Nq=n, Nk=k.shape[0], B=q_ptr.numel() - 1, H=self.H, Hk=self.Hk, d=self.d, causal=int(self.causal),
                      lam_f32=int(lam.dtype == torch.float32), dtype=DTYPES[q.dtype], max_q=self.max_q, max_k=self.max_k,
                      scale=self.scale)
         a.q_rs, a.q_hs, a.q_ms = q.stride()[:3]
@@ -115,7 +125,7 @@ class _Call:
         if train:
             rest = 0 if q.dtype == torch.float32 else n * self.H * self.d + 3
             kept = torch.empty(n * self.H * (2 * self.d + 2) + rest, dtype=torch.float32, device=dev)
-        self.args = a = self.block(q, k, v, lam, o, kept)
+        self.args = a = self.block(q, k, v, lam, o, kept, *self.segments())
         a.ws_floats = L.gps_diff_attn_fwd_workspace_floats(ctypes.addressof(a))
         ws = torch.empty(a.ws_floats, dtype=torch.float32, device=dev) if a.ws_floats else None
         a.ws = ptr(ws)
@@ -156,16 +166,17 @@ class _DiffAttention(torch.autograd.Function):
         q, k, v, lam = _chunked(q), _chunked(k), _chunked(v), lam.contiguous()
         o, kept = call.forward(q, k, v, lam, train)
         if train:
-            ctx.save_for_backward(q, k, v, lam, o, kept)
-            ctx.call, ctx.at = call, where(q, k, v, lam, o, kept)
+            saved = (q, k, v, lam, o, kept, *call.segments())
+            ctx.save_for_backward(*saved)
+            ctx.call, ctx.at = call, where(*saved)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, lam, o, kept = ctx.saved_tensors
+        saved = q, k, v, lam, *_ = ctx.saved_tensors
         dq, dk, dv = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v)]
         c = ctx.call
-        a = DiffAttn.from_buffer_copy(c.args) if where(q, k, v, lam, o, kept) == ctx.at else c.block(q, k, v, lam, o, kept)
+        a = DiffAttn.from_buffer_copy(c.args) if where(*saved) == ctx.at else c.block(*saved)
         dlam = c.backward(a, lam, do, dq, dk, dv)
         return dq, dk, dv, dlam, None, None
 
@@ -186,17 +197,17 @@ class _DiffSegmentAttention(torch.autograd.Function):
         qkv, lam = _chunked(qkv), lam.contiguous()
         o, kept = call.forward(*_split(qkv, call.H, call.Hk, call.d), lam, train)
         if train:
-            ctx.save_for_backward(qkv, lam, o, kept)
-            ctx.call, ctx.at = call, where(qkv, lam, o, kept)
+            saved = (qkv, lam, o, kept, *call.segments())
+            ctx.save_for_backward(*saved)
+            ctx.call, ctx.at = call, where(*saved)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        qkv, lam, o, kept = ctx.saved_tensors
+        saved = qkv, lam, *rest = ctx.saved_tensors
         c = ctx.call
         d_qkv = torch.empty_like(qkv, memory_format=torch.contiguous_format)
-        same = where(qkv, lam, o, kept) == ctx.at
-        a = DiffAttn.from_buffer_copy(c.args) if same else c.block(*_split(qkv, c.H, c.Hk, c.d), lam, o, kept)
+        a = DiffAttn.from_buffer_copy(c.args) if where(*saved) == ctx.at else c.block(*_split(qkv, c.H, c.Hk, c.d), lam, *rest)
         dlam = c.backward(a, lam, do, *_split(d_qkv, c.H, c.Hk, c.d))
         return d_qkv, dlam, None, None
 
@@ -218,7 +229,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     longest segment where the host knows it; they choose the launch shape only, and one query per segment
     (``max_q = 1``) over long key segments is split along the keys.
 
-    Differentiable once in ``q``, ``k``, ``v`` and ``lam``; results do not change from run to run."""
+    Differentiable once in ``q``, ``k``, ``v`` and ``lam``; results do not change from run to run.  The backward reads the offsets
+    and the mask again: one that was changed in place in between raises, like any saved tensor."""
     call = _Call(q, k, v, lam, q_ptr, k_ptr, causal, key_mask, scale, max_q, max_k)
     train = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam))
     return _DiffAttention.apply(q, k, v, lam, call, train)
