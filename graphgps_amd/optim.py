@@ -503,14 +503,10 @@ class FlatAdamW8bit(FlatAdamW):
     @torch.no_grad()
     def load_state_dict(self, sd) -> None:
         a = self.arena
-        for k, v in sd["param_groups"][0].items():
-            if k != "params":
-                self.param_groups[0][k] = v
-        self.param_groups[0].setdefault("max_grad_norm", None)
-        self.seed = int(sd.get("seed", self.seed))
-        steps = [0.0] * len(a.params)
-        for t in (self.exp_avg, self.exp_avg_sq, self.exp_avg_exp, self.exp_avg_sq_exp):
-            t.zero_()
+        group, seed = sd["param_groups"][0], int(sd.get("seed", self.seed))
+        if not 0 <= seed < 1 << 32:
+            raise ValueError(f"FlatAdamW8bit: seed {seed} is no 32-bit unsigned number")
+        steps, moments = [0.0] * len(a.params), []
         for i, (o, p, (b, nb)) in enumerate(zip(a.offsets, a.params, self._block_ranges())):
             st = sd["state"].get(i)
             if st is None:
@@ -522,13 +518,22 @@ class FlatAdamW8bit(FlatAdamW):
                     raise ValueError(f"FlatAdamW8bit: {name} of parameter {i} has {code.numel()} elements, not {k}")
                 if code.dtype == torch.uint8:
                     exp = st[name + "_exp"].reshape(-1)
-                    if exp.numel() != nb:
-                        raise ValueError(f"FlatAdamW8bit: {name}_exp of parameter {i} has {exp.numel()} blocks, not {nb}")
+                    if exp.numel() != nb or exp.dtype != torch.uint8:
+                        raise ValueError(f"FlatAdamW8bit: {name}_exp of parameter {i} has {exp.numel()} blocks of {exp.dtype}, not {nb} of uint8")
                 else:
                     code, exp = encode_moment(code.float(), octaves, self.block)
-                getattr(self, name)[o:o + k].copy_(code)
-                getattr(self, name + "_exp")[b:b + nb].copy_(exp)
+                moments += [(name, slice(o, o + k), code), (name + "_exp", slice(b, b + nb), exp)]
             steps[i] = float(st["step"])
+        # everything fits: only now does the optimizer change
+        for t in (self.exp_avg, self.exp_avg_sq, self.exp_avg_exp, self.exp_avg_sq_exp):
+            t.zero_()
+        for name, at, value in moments:
+            getattr(self, name)[at].copy_(value)
+        for k, v in group.items():
+            if k != "params":
+                self.param_groups[0][k] = v
+        self.param_groups[0].setdefault("max_grad_norm", None)
+        self.seed = seed
         self.param_step.copy_(torch.tensor(steps, dtype=torch.float32))
         self.hyper[6] = max(steps)
         self._hyper_host = None
