@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
                                                      const int64_t* __restrict__ chunk_off, const int32_t* __restrict__ chunk_len,
                                                      const int32_t* __restrict__ chunk_param, const uint8_t* __restrict__ active,
                                                      int64_t n_chunks, double* __restrict__ hyper, float* __restrict__ pstep,
-                                                     uint32_t seed, const float* __restrict__ ws, int n_ws,
+                                                     const uint32_t* __restrict__ seed, const float* __restrict__ ws, int n_ws,
                                                      const ChunkCoef* __restrict__ coef) {
   __shared__ double shd[kWaves];
   __shared__ Coef shk;
@@ -154,6 +154,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
   __syncthreads();
 
   const Coef k = shk;
+  const uint32_t seed0 = seed[0];
   for (int64_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int prm = chunk_param[c];
     if (!active[prm]) continue;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(float* __restrict__ p, cons
     if (threadIdx.x == 0 && (c == 0 || chunk_param[c - 1] != prm)) pstep[prm] = bc.step;
     const int64_t off = chunk_off[c];
     const int len = chunk_len[c];
-    const uint32_t key = mix32((uint32_t)(int64_t)bc.step * 0x9E3779B9u + seed);
+    const uint32_t key = mix32((uint32_t)(int64_t)bc.step * 0x9E3779B9u + seed0);
     const bool wide = ((reinterpret_cast<uintptr_t>(p + off) | reinterpret_cast<uintptr_t>(g + off)) & 15) == 0 &&
                       ((reinterpret_cast<uintptr_t>(m + off) | reinterpret_cast<uintptr_t>(v + off)) & 3) == 0;
     for (int b = wave; b * kBlock < len; b += kWaves) {
@@ -307,10 +308,10 @@ size_t gps_adamw8_workspace_floats(int64_t n_chunks) { return n_chunks > 0 ? (si
 
 int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, const int64_t* chunk_off,
                     const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active, int64_t n_chunks, double* hyper,
-                    float* pstep, uint32_t seed, float* ws, gps_stream_t stream) {
+                    float* pstep, const uint32_t* seed, float* ws, gps_stream_t stream) {
   GPS_REQUIRE(n_chunks >= 0 && n_chunks < (int64_t(1) << 31), "gps_adamw8_step: n_chunks=%lld", (long long)n_chunks);
   if (n_chunks == 0) return GPS_OK;
-  GPS_REQUIRE(p && g && m && v && m_exp && v_exp && chunk_off && chunk_len && chunk_param && active && hyper && pstep && ws,
+  GPS_REQUIRE(p && g && m && v && m_exp && v_exp && chunk_off && chunk_len && chunk_param && active && hyper && pstep && seed && ws,
               "gps_adamw8_step: null pointer argument");
   GPS_REQUIRE(gps_optim_chunk() == kChunk, "gps_adamw8_step: chunk table of %d elements", gps_optim_chunk());
   hipStream_t s = gps::as_stream(stream);

@@ -8,7 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from typing import Optional
 
 import torch  # noqa: F401  -- must be imported first: it maps the HIP runtime our .so binds to
@@ -16,7 +16,7 @@ import torch  # noqa: F401  -- must be imported first: it maps the HIP runtime o
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # GPS_HIP_LIB: an alternative build of the same ABI (A/B timing of kernel variants in one process launch each)
 LIB_PATH = os.environ.get("GPS_HIP_LIB") or os.path.join(_HERE, "csrc", "libgps_hip.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -137,7 +137,7 @@ _SIGNATURES = {
     "gps_sandwich_norm_bwd": (c_int, [_P, _P]),
     "gps_adamw8_block": (c_int, []),
     "gps_adamw8_workspace_floats": (c_size_t, [c_int64]),
-    "gps_adamw8_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P, _P, c_uint32, _P, _P]),
+    "gps_adamw8_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P, _P, _P, _P, _P]),
     "gps_adamw8_values": (c_int, [_P, _P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, _P, _P, _P]),
     "gps_seg_attn_bias_bwd": (c_int, [_P, _P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64,
                                       c_int, c_int, c_float, c_float, c_uint64, _P, _P, c_int64, _P, _P]),

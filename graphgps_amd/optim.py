@@ -403,7 +403,8 @@ class FlatAdamW8bit(FlatAdamW):
     A moment is a byte per element plus a power-of-two unit per block of 256 elements of a parameter (codes of three mantissa bits;
     include/gps_hip.h has the format).  Codes are rounded up or down at random so that the moving averages keep their mean; the
     random bits are a hash of (element, step, ``seed``), so a run repeats exactly.  Parameters, gradients and the update itself are
-    fp32.  A gradient that is not finite makes the moments of its whole block so.
+    fp32.  A gradient that is not finite makes the moments of its whole block so.  ``seed`` lives on the device beside the
+    hyper-parameters: a captured step goes on with the one that ``load_state_dict()`` brings.
 
     ``state_dict()`` holds the codes (uint8 ``exp_avg`` / ``exp_avg_sq`` in the parameter's shape, their blocks' ``*_exp``);
     ``load_state_dict()`` takes those, or the fp32 moments of :class:`FlatAdamW` / ``torch.optim.AdamW`` and rounds them to
@@ -411,10 +412,25 @@ class FlatAdamW8bit(FlatAdamW):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  max_grad_norm: Optional[float] = None, seed: int = 0):
+        self._check_seed(seed)
+        super().__init__(params, lr, betas, eps, weight_decay, max_grad_norm)
+        self._seed_word = torch.zeros(1, dtype=torch.int32, device=self.arena.device)
+        self.seed = seed
+
+    @staticmethod
+    def _check_seed(seed) -> int:
         if not 0 <= int(seed) < 1 << 32:
             raise ValueError(f"FlatAdamW8bit: seed {seed} is no 32-bit unsigned number")
-        super().__init__(params, lr, betas, eps, weight_decay, max_grad_norm)
-        self.seed = int(seed)
+        return int(seed)
+
+    @property
+    def seed(self) -> int:
+        return self._seed
+
+    @seed.setter
+    def seed(self, seed) -> None:
+        self._seed = self._check_seed(seed)
+        self._seed_word.fill_(self._seed - (1 << 32) if self._seed >= 1 << 31 else self._seed)
 
     def _alloc_state(self) -> None:
         a = self.arena
@@ -457,7 +473,7 @@ class FlatAdamW8bit(FlatAdamW):
             check(_lib.load().gps_adamw8_step(ptr(a.flat_p), ptr(a.flat_g), ptr(self.exp_avg), ptr(self.exp_avg_sq),
                                               ptr(self.exp_avg_exp), ptr(self.exp_avg_sq_exp), ptr(a.chunk_off), ptr(a.chunk_len),
                                               ptr(a.chunk_param), ptr(a.active), a.n_chunks, ptr(self.hyper), ptr(self.param_step),
-                                              self.seed, ptr(self._ws), current_stream(a.device)), "gps_adamw8_step")
+                                              ptr(self._seed_word), ptr(self._ws), current_stream(a.device)), "gps_adamw8_step")
 
     def moments(self, dtype: torch.dtype = torch.bfloat16):
         """``(exp_avg, exp_avg_sq)`` as numbers, in the arena's layout (``arena.offsets``); bfloat16 holds every value exactly."""
@@ -503,9 +519,7 @@ class FlatAdamW8bit(FlatAdamW):
     @torch.no_grad()
     def load_state_dict(self, sd) -> None:
         a = self.arena
-        group, seed = sd["param_groups"][0], int(sd.get("seed", self.seed))
-        if not 0 <= seed < 1 << 32:
-            raise ValueError(f"FlatAdamW8bit: seed {seed} is no 32-bit unsigned number")
+        group, seed = sd["param_groups"][0], self._check_seed(sd.get("seed", self.seed))
         steps, moments = [0.0] * len(a.params), []
         for i, (o, p, (b, nb)) in enumerate(zip(a.offsets, a.params, self._block_ranges())):
             st = sd["state"].get(i)

@@ -818,13 +818,14 @@ int gps_sandwich_norm_bwd(const gps_sandwich_norm* a, gps_stream_t stream);
  * offset, step = its parameter's step, mix(x): x ^= x >> 16, x *= 0x7feb352d, x ^= x >> 15, x *= 0x846ca68b, x ^= x >> 16:
  * the same run gives the same codes.
  *   m, v           uint8, the arena's layout;  m_exp, v_exp: uint8 [n_chunks * gps_optim_chunk() / gps_adamw8_block()]
+ *   seed           one word on the device, beside hyper: a captured step follows a checkpoint that is loaded into both
  *   ws             gps_adamw8_workspace_floats(n_chunks) floats; everything else as in gps_adamw_step
  * The parameter update uses the moments before they are rounded. */
 int gps_adamw8_block(void);
 size_t gps_adamw8_workspace_floats(int64_t n_chunks);
 int gps_adamw8_step(float* p, const float* g, uint8_t* m, uint8_t* v, uint8_t* m_exp, uint8_t* v_exp, const int64_t* chunk_off,
                     const int32_t* chunk_len, const int32_t* chunk_param, const uint8_t* active, int64_t n_chunks, double* hyper,
-                    float* pstep, uint32_t seed, float* ws, gps_stream_t stream);
+                    float* pstep, const uint32_t* seed, float* ws, gps_stream_t stream);
 /* The moments' values, arena layout, GPS_F32 or GPS_BF16 (which holds each exactly: four significant bits).  n_gaps pieces
  * (gap_off, gap_len <= gps_optim_chunk()) that belong to no parameter are set to zero.  Either output may be NULL. */
 int gps_adamw8_values(const uint8_t* m, const uint8_t* v, const uint8_t* m_exp, const uint8_t* v_exp, const int64_t* chunk_off,
