@@ -40,6 +40,7 @@ class GraphormerLayer(torch.nn.Module):
         )
         self.sandwich = bool(sandwich)
         if self.sandwich:
+            self.ctor_kwargs["sandwich"] = True
             self.attention_post_norm = torch.nn.LayerNorm(embed_dim)
             self.mlp_post_norm = torch.nn.LayerNorm(embed_dim)
             self.attention_gate = torch.nn.Parameter(torch.ones(embed_dim))
