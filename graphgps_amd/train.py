@@ -71,6 +71,13 @@ class _BackwardCut:
             torch.autograd.backward([v for v, _ in live], [g for _, g in live])
 
 
+def _fork_stream(cur):
+    """A stream beside ``cur`` of the same device.  torch hands out the 32 streams of its pool in turn, so that after 31 draws the next
+    one IS the capture's own stream, and a node that was forked onto it would not be forked."""
+    side = torch.cuda.Stream(device=cur.device)
+    return side if side.cuda_stream != cur.cuda_stream else torch.cuda.Stream(device=cur.device)
+
+
 class _Capture:
     """One hipGraph capture with the forked tick node every capture of a step carries (see ``TrainStep.capture``: a
     linear chain of several hundred kernel nodes on ONE stream faults at replay on this stack; one trivial forked node
@@ -91,7 +98,7 @@ class _Capture:
         self.open = True
         if self.tick is not None:
             cur = torch.cuda.current_stream(self.dev)
-            self.tside = torch.cuda.Stream(device=self.dev)
+            self.tside = _fork_stream(cur)
             self.tside.wait_stream(cur)
             with torch.cuda.stream(self.tside):
                 self.tick.add_(1.0)
@@ -521,7 +528,7 @@ def _capture_static(who, batch, dev, pool, body, before=None, tail=None):
             with torch.cuda.graph(graph, pool=pool, capture_error_mode="thread_local"):
                 if tick is not None:
                     cur = torch.cuda.current_stream(dev)
-                    tside = torch.cuda.Stream(device=dev)
+                    tside = _fork_stream(cur)
                     tside.wait_stream(cur)
                     with torch.cuda.stream(tside):
                         tick.add_(1.0)
