@@ -480,6 +480,9 @@ class FlatAdamW8bit(FlatAdamW):
         if dtype not in (torch.bfloat16, torch.float32):
             raise _lib.GpsHipError(f"FlatAdamW8bit.moments: {dtype} is neither bfloat16 nor float32")
         a = self.arena
+        if a.device.type != "cuda":
+            raise _lib.GpsHipError("FlatAdamW8bit.moments: parameters are on the CPU; their decoding is a HIP kernel (csrc/optim8.hip), "
+                                   "there is no CPU path")
         m = torch.empty(a.flat_p.numel(), dtype=dtype, device=a.device)
         v = torch.empty_like(m)
         with on_device(a.device):

@@ -76,3 +76,13 @@ def test_a_state_that_fits_is_taken_whole(fp32):
         for i in (0, 2):
             for k, v in sd["state"][i].items():
                 assert torch.equal(got["state"][i][k], v), (i, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_moments_of_cpu_parameters_are_refused(dtype):
+    """Its kernel would take their host pointers."""
+    from graphgps_amd.lib import GpsHipError
+    opt, g = make()
+    opt.load_state_dict(state_of(opt, g))
+    with pytest.raises(GpsHipError, match="on the CPU"):
+        opt.moments(dtype)
