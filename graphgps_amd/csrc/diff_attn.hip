@@ -10,15 +10,15 @@
 // In 16 bits a weight enters the second product in two terms, its rounding and what that lost (frag_lost).  The maps nearly cancel where
 // they agree, and a single rounding of each leaves its error on that small difference: relative to the value rounded once at the end, the
 // error of o is 1.0 times with two terms and 1.4 to 1.55 times with one on independent maps (0.0017 against 0.0025; two graphs of ~4,700
-// nodes 497 against 353 us, trees 14.5 against 11.7, ordered sequences 401 against 373), and 1 / (1 - lam) times and more where they
+// nodes 478 against 353 us, trees 14.1 against 11.7, ordered sequences 403 against 373), and 1 / (1 - lam) times and more where they
 // resemble each other.  Rounding the difference of the maps' weights instead needs the ratio of their final sums while it is formed: a
 // ratio from the keys seen so far puts errors into the sum that go by a key's weight when it was met, not by its weight at the end.
 //
 // Bound by the matrix units and what a SIMD issues around them: at 64 columns a block of 16 x 32 pairs is 40 matrix instructions (16
-// cycles each) and about 190 vector instructions, two exponentials per pair among them.  Two graphs of 4,175 and 5,261 nodes, 8 heads over
-// 4 of 64 columns, bf16: 497 us = 930 TFLOP/s of the products that the kernel makes (20 d flops per pair and head; 8 d are the
+// cycles each) and about 180 vector instructions, two exponentials per pair among them.  Two graphs of 4,175 and 5,261 nodes, 8 heads over
+// 4 of 64 columns, bf16: 478 us = 970 TFLOP/s of the products that the kernel makes (20 d flops per pair and head; 8 d are the
 // operator's), where a large matrix product reaches 1,262.  Four causal sequences of ~2,600 rows, 6 heads over 2 of 128 columns, fp16,
-// dropped keys: 401 us.  256 molecules of ~31 nodes, 8 heads of 24 columns, fp32: 42 us; 32 trees of ~123 nodes, 4 heads of 32, bf16: 14.5.
+// dropped keys: 403 us.  256 molecules of ~31 nodes, 8 heads of 24 columns, fp32: 42 us; 32 trees of ~123 nodes, 4 heads of 32, bf16: 14.1.
 #include <initializer_list>
 
 #include "diff_attn.hpp"
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (QT == 1 && DQ <= 64 ? 3 : 2)
 #pragma unroll
         for (int kk = 0; kk < BN / 32; ++kk) {
           p[m][i][kk] = frag_pack<T>(s[m][i][2 * kk], s[m][i][2 * kk + 1]);
-          if constexpr (sizeof(T) == 2) lost[m][i][kk] = frag_lost<T>(s[m][i][2 * kk], s[m][i][2 * kk + 1], p[m][i][kk]);
+          if constexpr (sizeof(T) == 2) lost[m][i][kk] = frag_lost(s[m][i][2 * kk], s[m][i][2 * kk + 1], p[m][i][kk]);
         }
       }
 #pragma unroll

@@ -90,11 +90,26 @@ __device__ __forceinline__ Frag<T> frag_pack(f32x4 a, f32x4 b) {
   }
   return f;
 }
-// what frag_pack lost, as a fragment of its own (16-bit types)
-template <typename T>
-__device__ __forceinline__ Frag<T> frag_lost(f32x4 a, f32x4 b, const Frag<T>& f) {
-  const vec_t<T, 4> x = __builtin_shufflevector(f.v, f.v, 0, 1, 2, 3), y = __builtin_shufflevector(f.v, f.v, 4, 5, 6, 7);
-  return frag_pack<T>(a - __builtin_convertvector(x, f32x4), b - __builtin_convertvector(y, f32x4));
+// what frag_pack lost, as a fragment of its own (16-bit types).  The two bfloat16 of a packed register are widened by a shift and a mask:
+// left to the compiler, each value is converted a second time first.
+__device__ __forceinline__ Frag<bf16> frag_lost(f32x4 a, f32x4 b, const Frag<bf16>& f) {
+  const vec_t<uint32_t, 4> w = __builtin_bit_cast(vec_t<uint32_t, 4>, f.v);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    a[2 * j] -= __uint_as_float(w[j] << 16);
+    a[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+    b[2 * j] -= __uint_as_float(w[2 + j] << 16);
+    b[2 * j + 1] -= __uint_as_float(w[2 + j] & 0xffff0000u);
+  }
+  return frag_pack<bf16>(a, b);
+}
+__device__ __forceinline__ Frag<f16> frag_lost(f32x4 a, f32x4 b, const Frag<f16>& f) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    a[j] -= (float)f.v[j];
+    b[j] -= (float)f.v[4 + j];
+  }
+  return frag_pack<f16>(a, b);
 }
 // A fragment of the TRANSPOSE of the row-major LDS tile `m` (row stride `ld`): row of A = column col0 + (l & 15), slots = rows
 // row0 .. row0 + 31 in frag_pack's order

@@ -300,8 +300,8 @@ __device__ __forceinline__ void dkv(const Args& a, const float* __restrict__ del
       ds[0][i] = frag_pack<T>(s[0][i][0], s[0][i][1]);
       ds[1][i] = frag_pack<T>(s[1][i][0], s[1][i][1]);
       if constexpr (two_terms<T, DQ>()) {
-        lost[0][i] = frag_lost<T>(s[0][i][0], s[0][i][1], ds[0][i]);
-        lost[1][i] = frag_lost<T>(s[1][i][0], s[1][i][1], ds[1][i]);
+        lost[0][i] = frag_lost(s[0][i][0], s[0][i][1], ds[0][i]);
+        lost[1][i] = frag_lost(s[1][i][0], s[1][i][1], ds[1][i]);
       }
     }
 #pragma unroll
@@ -514,7 +514,7 @@ __device__ __forceinline__ void dq(const Args& a, const float* __restrict__ delt
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
         ds[i] = frag_pack<T>(s[m][i][0], s[m][i][1]);
-        if constexpr (two_terms<T, DQ>()) lost[i] = frag_lost<T>(s[m][i][0], s[m][i][1], ds[i]);
+        if constexpr (two_terms<T, DQ>()) lost[i] = frag_lost(s[m][i][0], s[m][i][1], ds[i]);
       }
 #pragma unroll
       for (int c = 0; c < DQT; ++c) {

@@ -136,8 +136,8 @@ __global__ __launch_bounds__(kUnitWaves * 64, sizeof(T) * DQ <= 128 ? 2 : 1) voi
       const Frag<T> p0 = frag_pack<T>(s[0][0], s[0][1]), p1 = frag_pack<T>(s[1][0], s[1][1]);
       Frag<T> lost0, lost1;   // weights in two terms, as in diff_attn.hip
       if constexpr (sizeof(T) == 2) {
-        lost0 = frag_lost<T>(s[0][0], s[0][1], p0);
-        lost1 = frag_lost<T>(s[1][0], s[1][1], p1);
+        lost0 = frag_lost(s[0][0], s[0][1], p0);
+        lost1 = frag_lost(s[1][0], s[1][1], p1);
       }
 #pragma unroll
       for (int x = 0; x < DVT; ++x) {
