@@ -6,8 +6,8 @@
 // P_i is recomputed from the saved log-sum-exp.  k_diff_delta forms D; k_diff_bwd has workgroups that own keys and walk the
 // queries and workgroups that own queries and walk the keys (the scores and dP twice, but no atomics: every sum in one fixed order).
 //
-// Two graphs of 4,175 and 5,261 nodes, 8 heads over 4 of 64 columns, bf16: 1.17 ms = 550 TFLOP/s of its 28 d flops per pair and head (20 d
-// with the scores and dP once).  No unit is saturated: LDS 42 % busy (every fragment that a wavefront reads there serves one 16 x 16
+// Two graphs of 4,175 and 5,261 nodes, 8 heads over 4 of 64 columns, bf16: 1.04 ms in a replayed graph = 620 TFLOP/s of its 28 d flops per
+// pair and head (20 d with the scores and dP once), 1.17 under a tracer, as the figures below were taken.  No unit is saturated: LDS 42 % busy (every fragment that a wavefront reads there serves one 16 x 16
 // tile), vector units 40 %, matrix units 27 %; 213 registers leave two wavefronts per SIMD, which wait for each other's phases.
 // Tried and slower: two tiles per wavefront (373 registers, one wavefront per SIMD: 1.51 ms; for dQ alone, spilling: 1.44), three
 // wavefronts per SIMD (28 registers spilled: 1.29), eight wavefronts per workgroup (half the staging: 1.18-1.22), a copy of the step
@@ -19,9 +19,9 @@ namespace {
 
 // dS in two 16-bit terms.  With one, the error of dQ and dK is 1.41 to 1.5 times that of a gradient that is rounded once at its end, and
 // more (up to 1.9) where heads are narrow and rows see few keys: the terms of a sum cancel and their errors do not.  Up to 32
-// columns, where both second products of dS are small, it is kept in two: 1.1 to 1.3 times, for 20.6 us instead of 18.5 on 32 trees of ~123
-// nodes and 503 instead of 456 for a whole pass over 9 causal graphs of 2,108 (4 heads over 1, 16 columns).  Above that in one: two graphs of
-// ~4,700 nodes, 64 columns, would take 1,350 us instead of 1,180.
+// columns, where both second products of dS are small, it is kept in two: 1.0 to 1.1 times, for 39.8 us instead of 38.6 for a whole pass
+// over 32 trees of ~123 nodes and 523 instead of 487 over 9 causal graphs of 2,108 (4 heads over 1, 16 columns).  Above that in one: the
+// backward of two graphs of ~4,700 nodes, 64 columns, would take 1,165 us instead of 1,060.
 template <typename T, int DQ>
 constexpr bool two_terms() { return sizeof(T) == 2 && DQ == 32; }
 
